@@ -3,10 +3,12 @@
 #include "bucket.hpp"
 #include "fmx_internal.hpp"
 #include "moe.hpp"
+#include "paged.hpp"
 #include "prefill.hpp"
 
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <mutex>
 #include <thread>
@@ -170,6 +172,48 @@ void consume_fault(int fault) {
 }
 
 int fault_gate() { return g_fault.load() == FMX_FAULT_DEVICE_LOSS ? FMX_ERR_DEVICE_LOSS : FMX_OK; }
+
+// What the reads of a row of `width` elements need: whole 16-byte pieces.
+static bool row_stride_ok(uint64_t stride, uint64_t width, uint32_t element) {
+    return stride >= width && stride * element % 16 == 0 && stride < (uint64_t{1} << 40);
+}
+
+int prepare_paged(const fmx_paged_cache *cache, const fmx_paged_batch *batch, PagedArgs *a) {
+    if (!cache || !batch) return FMX_ERR_INVALID_ARGUMENT;
+    const uint32_t element = element_bytes(cache->type);
+    if (element == 0) return FMX_ERR_UNSUPPORTED_QUANTISATION;
+    if (!cache->k || !cache->v || !aligned16(cache->k) || !aligned16(cache->v)) return FMX_ERR_INVALID_ARGUMENT;
+    if (cache->kv_heads == 0 || cache->kv_heads > 65535 || cache->head_dim == 0 || cache->head_dim > 256 ||
+        cache->head_dim % 8 || cache->page_size == 0 || cache->page_size > 65536 || cache->pages == 0)
+        return FMX_ERR_SHAPE_MISMATCH;
+    if (!row_stride_ok(cache->page_stride, cache->head_dim, element) ||
+        !row_stride_ok(cache->position_stride, cache->head_dim, element) ||
+        !row_stride_ok(cache->head_stride, cache->head_dim, element))
+        return FMX_ERR_SHAPE_MISMATCH;
+    if (batch->tokens > 0x7fffffffu || batch->sequences > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
+    const uint64_t positions = static_cast<uint64_t>(batch->table_stride) * cache->page_size;
+    a->tokens = batch->sequences == 0 || batch->max_new == 0 ? 0 : batch->tokens;
+    if (a->tokens == 0) return FMX_OK;
+    if (!batch->starts || !batch->lengths || !batch->table) return FMX_ERR_INVALID_ARGUMENT;
+    if (batch->table_stride == 0) return FMX_ERR_SHAPE_MISMATCH;
+    a->k = static_cast<const uint8_t *>(cache->k);
+    a->v = static_cast<const uint8_t *>(cache->v);
+    a->page_bytes = cache->page_stride * element;
+    a->position_bytes = cache->position_stride * element;
+    a->head_bytes = cache->head_stride * element;
+    a->kv_heads = cache->kv_heads;
+    a->head_dim = cache->head_dim;
+    a->pages = cache->pages;
+    a->page = FastDiv(cache->page_size);
+    a->sequences = batch->sequences;
+    a->max_new = batch->max_new < batch->tokens ? batch->max_new : batch->tokens;
+    a->table_stride = batch->table_stride;
+    a->max_length = positions < 0x7fffffffu ? static_cast<uint32_t>(positions) : 0x7fffffffu;
+    a->starts = batch->starts;
+    a->lengths = batch->lengths;
+    a->table = batch->table;
+    return FMX_OK;
+}
 
 int status_of_hip(hipError_t e) {
     switch (e) {
@@ -609,8 +653,127 @@ int fmx_attention_decode(const float *q, const float *kv, uint64_t row_stride, u
                             static_cast<uint32_t *>(workspace), static_cast<hipStream_t>(stream));
 }
 
+// ---------------------------------------------------------- paged cache --
+
+int fmx_rope_frequencies(const fmx_rope_scaling *scaling, uint32_t dims, double *inv_freq, double *magnitude) {
+    if (!scaling || !inv_freq || !magnitude) return FMX_ERR_INVALID_ARGUMENT;
+    if (dims == 0 || dims % 2 || dims > 256) return FMX_ERR_SHAPE_MISMATCH;
+    const fmx_rope_scaling &c = *scaling;
+    if (!(c.base > 1.0) || !std::isfinite(c.base) || c.kind > FMX_ROPE_SCALE_BANDS) return FMX_ERR_INVALID_ARGUMENT;
+    if (c.kind != FMX_ROPE_SCALE_NONE && (!(c.factor >= 1.0) || !std::isfinite(c.factor)))
+        return FMX_ERR_INVALID_ARGUMENT;
+    if (c.kind == FMX_ROPE_SCALE_YARN || c.kind == FMX_ROPE_SCALE_BANDS)
+        if (!(c.context > 0.0) || !(c.low > 0.0) || !(c.high > c.low) || !std::isfinite(c.context) || !std::isfinite(c.high))
+            return FMX_ERR_INVALID_ARGUMENT;
+    const double two_pi = 6.283185307179586476925;
+    *magnitude = c.kind == FMX_ROPE_SCALE_YARN ? 0.1 * std::log(c.factor) + 1.0 : 1.0;
+    // the pair that turns n times over the trained context
+    const auto pair_of = [&](double n) {
+        return dims * std::log(c.context / (n * two_pi)) / (2.0 * std::log(c.base));
+    };
+    double first = 0.0, last = 0.0;
+    if (c.kind == FMX_ROPE_SCALE_YARN) {
+        first = std::fmax(0.0, std::floor(pair_of(c.high)));
+        last = std::fmin(dims - 1.0, std::ceil(pair_of(c.low)));
+    }
+    for (uint32_t i = 0; i < dims / 2; ++i) {
+        const double f = std::pow(c.base, -2.0 * i / dims), slow = f / c.factor;
+        switch (c.kind) {
+        case FMX_ROPE_SCALE_LINEAR: inv_freq[i] = slow; break;
+        case FMX_ROPE_SCALE_YARN: {
+            const double ramp = std::fmin(1.0, std::fmax(0.0, (i - first) / std::fmax(last - first, 0.001)));
+            inv_freq[i] = slow * ramp + f * (1.0 - ramp);
+            break;
+        }
+        case FMX_ROPE_SCALE_BANDS: {
+            // turns over the trained context, between the low and the high factor
+            const double blend = std::fmin(1.0, std::fmax(0.0, (c.context * f / two_pi - c.low) / (c.high - c.low)));
+            inv_freq[i] = slow * (1.0 - blend) + f * blend;
+            break;
+        }
+        default: inv_freq[i] = f;
+        }
+    }
+    return FMX_OK;
+}
+
+int fmx_rope_append(const fmx_paged_cache *cache, const fmx_paged_batch *batch, const fmx_rope *rope, uint32_t heads,
+                    uint32_t in_type, const void *q, uint64_t q_stride, const void *k, uint64_t k_stride,
+                    const void *v, uint64_t v_stride, void *q_out, uint64_t q_out_stride, void *workspace,
+                    uint64_t workspace_bytes, void *stream) {
+    if (int rc = fault_gate()) return rc;
+    PagedArgs a;
+    if (int rc = prepare_paged(cache, batch, &a)) return rc;
+    if (!rope || rope->layout > FMX_ROPE_HALF || !std::isfinite(rope->magnitude)) return FMX_ERR_INVALID_ARGUMENT;
+    if (in_type != FMX_TYPE_F32 && in_type != cache->type) return FMX_ERR_UNSUPPORTED_QUANTISATION;
+    if (heads == 0 || heads > 65535 || rope->dims % 2 || rope->dims > cache->head_dim) return FMX_ERR_SHAPE_MISMATCH;
+    if (a.tokens == 0) return FMX_OK;
+    if (!q || !k || !v || !q_out || !workspace || workspace_bytes < kStatusBytes || (rope->dims && !rope->inv_freq))
+        return FMX_ERR_INVALID_ARGUMENT;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(workspace))
+        return FMX_ERR_INVALID_ARGUMENT;
+    const uint32_t in = element_bytes(in_type);
+    const uint64_t q_width = static_cast<uint64_t>(heads) * a.head_dim, kv_width = static_cast<uint64_t>(a.kv_heads) * a.head_dim;
+    if (!row_stride_ok(q_stride, q_width, in) || !row_stride_ok(k_stride, kv_width, in) ||
+        !row_stride_ok(v_stride, kv_width, in) || !row_stride_ok(q_out_stride, q_width, element_bytes(cache->type)))
+        return FMX_ERR_SHAPE_MISMATCH;
+    // a row of q_out inside q's must be the row itself
+    if (q == q_out && (in_type != cache->type || q_stride != q_out_stride)) return FMX_ERR_INVALID_ARGUMENT;
+    const RopeCall c{heads, in_type, q, k, v, q_stride, k_stride, v_stride, q_out, q_out_stride,
+                     static_cast<uint32_t *>(workspace)};
+    return rope_append(a, cache->type, *rope, c, static_cast<hipStream_t>(stream));
+}
+
+uint64_t fmx_attention_paged_workspace_bytes(const fmx_paged_cache *cache, const fmx_paged_batch *batch, uint32_t heads) {
+    PagedArgs a;
+    if (prepare_paged(cache, batch, &a) || heads == 0 || heads > 65535 || heads % cache->kv_heads) return 0;
+    return kStatusBytes + (a.tokens ? attention_paged_scratch(a, cache->type, heads) : 0);
+}
+
+int fmx_attention_paged(const fmx_paged_cache *cache, const fmx_paged_batch *batch, const fmx_attention_options *options,
+                        uint32_t heads, const void *q, uint64_t q_stride, uint32_t out_type, void *out,
+                        uint64_t out_stride, void *workspace, uint64_t workspace_bytes, void *stream) {
+    if (int rc = fault_gate()) return rc;
+    PagedArgs a;
+    if (int rc = prepare_paged(cache, batch, &a)) return rc;
+    if (!options || !std::isfinite(options->scale) || !(options->softcap >= 0.0) || !std::isfinite(options->softcap))
+        return FMX_ERR_INVALID_ARGUMENT;
+    if (out_type != FMX_TYPE_F32 && out_type != cache->type) return FMX_ERR_UNSUPPORTED_QUANTISATION;
+    if (heads == 0 || heads > 65535 || heads % cache->kv_heads) return FMX_ERR_SHAPE_MISMATCH;
+    if (a.tokens == 0) return FMX_OK;
+    if (static_cast<uint64_t>(a.tokens) * heads > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
+    if (!q || !out || !workspace || !aligned16(q) || !aligned16(out) || !aligned16(workspace))
+        return FMX_ERR_INVALID_ARGUMENT;
+    const uint64_t width = static_cast<uint64_t>(heads) * a.head_dim;
+    if (!row_stride_ok(q_stride, width, element_bytes(cache->type)) ||
+        !row_stride_ok(out_stride, width, element_bytes(out_type)))
+        return FMX_ERR_SHAPE_MISMATCH;
+    if (workspace_bytes < kStatusBytes + attention_paged_scratch(a, cache->type, heads)) return FMX_ERR_INVALID_ARGUMENT;
+    const AttentionCall c{heads, out_type, q, q_stride, out, out_stride, *options, static_cast<uint32_t *>(workspace),
+                          static_cast<uint8_t *>(workspace) + kStatusBytes};
+    return attention_paged(a, cache->type, c, static_cast<hipStream_t>(stream));
+}
+
+// ------------------------------------------------------------- sampling --
+
+uint64_t fmx_sample_workspace_bytes(uint32_t rows, uint32_t vocab) { return kStatusBytes + sample_scratch(rows, vocab); }
+
+int fmx_sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const fmx_sampling *sampling,
+               const float *uniform, uint32_t *ids, float *probs, void *workspace, uint64_t workspace_bytes,
+               void *stream) {
+    if (int rc = fault_gate()) return rc;
+    if (!sampling) return FMX_ERR_INVALID_ARGUMENT;
+    if (vocab == 0 || vocab > kSampleMaxVocab || row_stride < vocab || rows > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
+    if (rows == 0) return FMX_OK;
+    if (!logits || !uniform || !ids || !workspace || !aligned16(workspace)) return FMX_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(logits) & 3u) return FMX_ERR_INVALID_ARGUMENT;
+    if (workspace_bytes < kStatusBytes + sample_scratch(rows, vocab)) return FMX_ERR_INVALID_ARGUMENT;
+    return sample(logits, row_stride, rows, vocab, *sampling, uniform, ids, probs, static_cast<uint32_t *>(workspace),
+                  static_cast<uint8_t *>(workspace) + kStatusBytes, static_cast<hipStream_t>(stream));
+}
+
 int fmx_moe_status_of(uint32_t word) {
-    if (word & STATUS_BAD_EXPERT) return FMX_ERR_INVALID_ARGUMENT;
+    if (word & (STATUS_BAD_EXPERT | STATUS_BAD_PAGE)) return FMX_ERR_INVALID_ARGUMENT;
     if (word & STATUS_NONFINITE_SCORE) return FMX_ERR_INTERNAL;
     return FMX_OK;
 }

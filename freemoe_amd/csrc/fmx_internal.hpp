@@ -66,7 +66,7 @@ int packed_geometry(uint32_t type_id, uint32_t rows, uint32_t cols, PackedGeomet
 int raw_geometry(uint32_t type_id, uint32_t *block_size, uint32_t *block_bytes);
 
 // Device error word bits (fmx_moe_status).
-enum : uint32_t { STATUS_NONFINITE_SCORE = 1u, STATUS_BAD_EXPERT = 2u };
+enum : uint32_t { STATUS_NONFINITE_SCORE = 1u, STATUS_BAD_EXPERT = 2u, STATUS_BAD_PAGE = 4u };
 
 // ---------------------------------------------------------------- device --
 

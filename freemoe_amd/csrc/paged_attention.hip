@@ -1,0 +1,506 @@
+// paged_attention.hip — attention of a batch's new tokens over the pages their
+// sequences hold.
+//
+// Query head h of the token at position p, over the visible positions j of its
+// sequence (j <= p, and p - j < window where there is one):
+//   s_j = scale q . k_j  (softcap c: c tanh(s_j / c)),
+//   out = sum_j e^(s_j - m) v_j / (sum_j e^(s_j - m) + e^(sink_h - m)),
+// in one pass over j with the running maximum m and sum: where a later tile
+// raises m, what was summed is multiplied by e^(m_old - m_new). Scores are kept
+// in units of log 2 (scale times log2 e), so that e^x is one v_exp_f32.
+//
+// The query heads of one kv head read the same keys: a sequence's new tokens
+// times those heads are the rows of one small matrix, row r being token r /
+// group and head r % group.
+#include "paged.hpp"
+
+namespace fmx {
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr uint32_t kWaves = 4;
+constexpr uint32_t kThreads = 64 * kWaves;
+
+struct AttentionArgs {
+    PagedArgs a;
+    const uint8_t *q;
+    uint8_t *out;
+    uint64_t q_bytes, out_bytes; // row strides
+    uint32_t heads;
+    FastDiv group;               // query heads of a kv head
+    float scale;                 // times log2 e (softcap: 1 / softcap times the plain one)
+    float softcap;               // times log2 e, or 0
+    uint32_t window;             // 0x80000000 where there is none
+    const float *sinks;
+    uint32_t out_type;
+    uint32_t *status;
+};
+
+// Element types: how many 16-bit parts carry a weight to f32 accuracy, and the
+// power of two the weights are kept at. A half's range ends at 2^-24, which
+// would cost small weights their low bits: its weights are kept 2^15 times as
+// large (at most 32768; the sum carries the same factor).
+template <typename T> struct Element;
+template <> struct Element<float> { static constexpr int kParts = 1; static constexpr float kLift = 0.0f; };
+template <> struct Element<_Float16> {
+    static constexpr int kParts = 2;
+    static constexpr float kLift = 15.0f;
+    static constexpr uint32_t kExponent = 0x7c007c00u;
+};
+template <> struct Element<__bf16> {
+    static constexpr int kParts = 3;
+    static constexpr float kLift = 0.0f;
+    static constexpr uint32_t kExponent = 0x7f807f80u;
+};
+
+template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
+
+__device__ __forceinline__ f32x4 mma16(Vec8<__bf16>::type a, Vec8<__bf16>::type b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(Vec8<_Float16>::type a, Vec8<_Float16>::type b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A row's maximum or sum over the four 16-lane groups that hold its keys.
+__device__ __forceinline__ float row_max(float v) {
+    uint32_t a, b;
+    lane_pair_u32<16>(__builtin_bit_cast(uint32_t, v), a, b);
+    v = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    lane_pair_u32<32>(__builtin_bit_cast(uint32_t, v), a, b);
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    uint32_t a, b;
+    lane_pair_u32<16>(__builtin_bit_cast(uint32_t, v), a, b);
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    lane_pair_u32<32>(__builtin_bit_cast(uint32_t, v), a, b);
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// One wavefront's 16 rows against kKeys keys, everything in registers: the
+// scores are formed transposed (keys x rows), so that lane (c = lane % 16, g =
+// lane / 16) holds row c's scores of the keys the next product wants from it,
+// and the weights never move. The keys' order inside a product's k dimension
+// is free as long as both operands agree: slot 8 g + x of the 32 is key 4 g + x
+// (x < 4) or 16 + 4 g + x - 4, as the score registers have them.
+// Keys and values come straight from global memory: a lane loads 16 bytes of
+// key c per step, and of the 8 keys of its slots kE = DP / 16 consecutive
+// elements, from kE c on: value product m has element kE c + m in its row c, so
+// the transposition is one v_perm per two elements and whole rows are read.
+template <typename T, int DP> struct Tile16 {
+    static constexpr int kKeys = 32, kScores = 8, kE = DP / 16, kSteps = DP / 32;
+    static constexpr int kLoads = kE * 2 / 16 ? kE * 2 / 16 : 1; // 16-byte (or one 8-byte) pieces of a value row
+    typedef typename Vec8<T>::type v8;
+    v8 q[kSteps], k[2][kSteps];
+    uint32_t v[kScores][kE / 2];
+    f32x4 acc[kE];
+
+    static __device__ __forceinline__ uint32_t key(uint32_t g, int x) { return (x < 4 ? 0 : 12) + 4 * g + x; }
+
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t g, uint32_t D) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] = v8{};
+            if (32 * s + 8 * g < D) q[s] = __builtin_bit_cast(v8, ld16(row + (32 * s + 8 * g) * 2));
+        }
+    }
+    __device__ __forceinline__ void load(const uint8_t *kp, const uint8_t *vp, const uint64_t *offset, uint32_t c,
+                                         uint32_t g, uint32_t D) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint8_t *row = kp + offset[16 * t + c] + 16 * g;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (D != DP) k[t][s] = v8{};
+                if (D == DP || 32 * s + 8 * g < D) k[t][s] = __builtin_bit_cast(v8, ld16(row + 64 * s));
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < kScores; ++x) {
+            const uint8_t *row = vp + offset[key(g, x)] + kE * 2 * c;
+            if constexpr (kE == 4) {
+                uint2 w = make_uint2(0, 0);
+                if (D == DP || kE * c < D) w = ld8(row);
+                v[x][0] = w.x;
+                v[x][1] = w.y;
+            } else {
+#pragma unroll
+                for (int h = 0; h < kLoads; ++h) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (D == DP || kE * c + 8 * h < D) w = ld16(row + 16 * h);
+                    v[x][4 * h] = w.x;
+                    v[x][4 * h + 1] = w.y;
+                    v[x][4 * h + 2] = w.z;
+                    v[x][4 * h + 3] = w.w;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void scores(float *s) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) r = mma16(k[t][i], q[i], r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * t + i] = r[i];
+        }
+    }
+    __device__ __forceinline__ void clear_values(uint32_t g, uint32_t first_hidden) {
+#pragma unroll
+        for (int x = 0; x < kScores; ++x)
+            if (key(g, x) >= first_hidden)
+#pragma unroll
+                for (int w = 0; w < kE / 2; ++w) v[x][w] = 0;
+    }
+    static __device__ __forceinline__ v8 columns(const uint32_t (&w)[kScores][kE / 2], int m) {
+        u32x4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            r[j] = __builtin_amdgcn_perm(w[2 * j + 1][m / 2], w[2 * j][m / 2], m % 2 ? 0x07060302u : 0x05040100u);
+        return __builtin_bit_cast(v8, r);
+    }
+    template <int kParts> __device__ __forceinline__ void add(const float *p) {
+        float rest[kScores];
+#pragma unroll
+        for (int x = 0; x < kScores; ++x) rest[x] = p[x];
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+            v8 w;
+#pragma unroll
+            for (int x = 0; x < kScores; ++x) {
+                w[x] = static_cast<T>(rest[x]);
+                if (part + 1 < kParts) rest[x] -= static_cast<float>(w[x]); // exact
+            }
+#pragma unroll
+            for (int m = 0; m < kE; ++m) acc[m] = mma16(columns(v, m), w, acc[m]);
+        }
+    }
+    // Infinities and NaN among the values of a tile that some row sees only in
+    // part: a zero weight would not keep them out of that row's sums. They leave
+    // the values, and the sums of the rows that see one become NaN, found by a
+    // product of 0 / 1 matrices.
+    __device__ __forceinline__ void split_nonfinite(const bool *seen) {
+        constexpr uint32_t kHalf = Element<T>::kExponent & 0xffffu, kOne = sizeof(T) == 2 && kHalf == 0x7f80 ? 0x3f80 : 0x3c00;
+        bool any = false;
+#pragma unroll
+        for (int x = 0; x < kScores; ++x)
+#pragma unroll
+            for (int w = 0; w < kE / 2; ++w)
+                any |= (v[x][w] & kHalf) == kHalf || (v[x][w] >> 16 & kHalf) == kHalf;
+        if (!__any(any)) return;
+        uint32_t odd[kScores][kE / 2];
+#pragma unroll
+        for (int x = 0; x < kScores; ++x)
+#pragma unroll
+            for (int w = 0; w < kE / 2; ++w) {
+                odd[x][w] = 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if ((v[x][w] >> (16 * h) & kHalf) == kHalf) {
+                        odd[x][w] |= kOne << (16 * h);
+                        v[x][w] &= ~(0xffffu << (16 * h));
+                    }
+            }
+        v8 w;
+#pragma unroll
+        for (int x = 0; x < kScores; ++x) w[x] = static_cast<T>(seen[x] ? 1.0f : 0.0f);
+#pragma unroll
+        for (int m = 0; m < kE; ++m) {
+            const f32x4 n = mma16(columns(odd, m), w, f32x4{});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][i] = n[i] > 0.0f ? __builtin_nanf("") : acc[m][i];
+        }
+    }
+};
+
+// The same on v_mfma_f32_16x16x4_f32, 16 keys at a time: product i of a score
+// step takes element 16 s + 4 g + i of key c, product i of the values slot g =
+// key 4 g + i.
+template <int DP> struct Tile16<float, DP> {
+    static constexpr int kKeys = 16, kScores = 4, kE = DP / 16, kSteps = DP / 16;
+    f32x4 q[kSteps], k[kSteps], v[kScores][kE / 4], acc[kE];
+
+    static __device__ __forceinline__ uint32_t key(uint32_t g, int x) { return 4 * g + x; }
+
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t g, uint32_t D) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] = f32x4{};
+            if (16 * s + 4 * g < D) q[s] = __builtin_bit_cast(f32x4, ld16(row + (16 * s + 4 * g) * 4));
+        }
+    }
+    __device__ __forceinline__ void load(const uint8_t *kp, const uint8_t *vp, const uint64_t *offset, uint32_t c,
+                                         uint32_t g, uint32_t D) {
+        const uint8_t *row = kp + offset[c] + 16 * g;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (D != DP) k[s] = f32x4{};
+            if (D == DP || 16 * s + 4 * g < D) k[s] = __builtin_bit_cast(f32x4, ld16(row + 64 * s));
+        }
+#pragma unroll
+        for (int x = 0; x < kScores; ++x) {
+            const uint8_t *from = vp + offset[key(g, x)] + kE * 4 * c;
+#pragma unroll
+            for (int h = 0; h < kE / 4; ++h) {
+                if (D != DP) v[x][h] = f32x4{};
+                if (D == DP || kE * c + 4 * h < D) v[x][h] = __builtin_bit_cast(f32x4, ld16(from + 16 * h));
+            }
+        }
+    }
+    __device__ __forceinline__ void scores(float *s) const {
+        f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][i], q[t][i], r, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = r[i];
+    }
+    __device__ __forceinline__ void clear_values(uint32_t g, uint32_t first_hidden) {
+#pragma unroll
+        for (int x = 0; x < kScores; ++x)
+            if (key(g, x) >= first_hidden)
+#pragma unroll
+                for (int h = 0; h < kE / 4; ++h) v[x][h] = f32x4{};
+    }
+    template <int kParts> __device__ __forceinline__ void add(const float *p) {
+#pragma unroll
+        for (int m = 0; m < kE; ++m)
+#pragma unroll
+            for (int x = 0; x < kScores; ++x)
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][m / 4][m % 4], p[x], acc[m], 0, 0, 0);
+    }
+    __device__ __forceinline__ void split_nonfinite(const bool *seen) {
+        bool any = false;
+#pragma unroll
+        for (int x = 0; x < kScores; ++x)
+#pragma unroll
+            for (int m = 0; m < kE; ++m) any |= !__builtin_isfinite(v[x][m / 4][m % 4]);
+        if (!__any(any)) return;
+#pragma unroll
+        for (int m = 0; m < kE; ++m) {
+            f32x4 n = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int x = 0; x < kScores; ++x) {
+                const bool finite = __builtin_isfinite(v[x][m / 4][m % 4]);
+                n = __builtin_amdgcn_mfma_f32_16x16x4f32(finite ? 0.0f : 1.0f, seen[x] ? 1.0f : 0.0f, n, 0, 0, 0);
+                if (!finite) v[x][m / 4][m % 4] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][i] = n[i] > 0.0f ? __builtin_nanf("") : acc[m][i];
+        }
+    }
+};
+
+// A score in units of log 2 from q . k.
+__device__ __forceinline__ float log2_score(const AttentionArgs &A, float dot) {
+    const float s = dot * A.scale;
+    return A.softcap != 0.0f ? tanhf(s) * A.softcap : s;
+}
+
+__device__ __forceinline__ void store4(uint8_t *row, uint32_t d, uint32_t type, f32x4 x) {
+    if (type == FMX_TYPE_F32) {
+        *reinterpret_cast<f32x4 *>(row + d * 4) = x;
+    } else if (type == FMX_TYPE_F16) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<h4 *>(row + d * 2) = __builtin_convertvector(x, h4);
+    } else {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<b4 *>(row + d * 2) = __builtin_convertvector(x, b4);
+    }
+}
+
+constexpr uint32_t kRows = 16;
+
+// 16 rows of one sequence and kv head per workgroup; its wavefronts take tiles
+// of keys in turn and join their sums through LDS.
+// grid: row tiles x kv heads, the heads fastest.
+template <typename T, int DP, int kParts>
+__global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs A) {
+    using Tile = Tile16<T, DP>;
+    constexpr float kLift = Element<T>::kLift;
+    constexpr uint32_t kStride = DP + 4;
+    extern __shared__ __align__(16) char lds[];
+    float *sums = reinterpret_cast<float *>(lds); // [waves][rows][kStride]
+    __shared__ __align__(16) uint64_t offsets[kWaves][32];
+    __shared__ float top_s[kWaves][kRows], mass_s[kWaves][kRows];
+    const PagedArgs &a = A.a;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, target = blockIdx.x / a.kv_heads, G = A.group.d, D = a.head_dim;
+    uint32_t index, item;
+    Sequence seq;
+    bool bad = false;
+    const bool found = find_item(
+        a, target, [&](const Sequence &s) { return (s.count * G + kRows - 1) / kRows; }, index, seq, item, bad);
+    if (!found) {
+        if (bad && tid == 0) atomicOr(A.status, STATUS_BAD_PAGE);
+        return;
+    }
+    const uint32_t rows = seq.count * G, r0 = item * kRows, r1 = r0 + kRows < rows ? r0 + kRows : rows;
+    const int32_t before = static_cast<int32_t>(seq.length) - static_cast<int32_t>(seq.count);
+    const int32_t p_first = before + static_cast<int32_t>(A.group.div(r0));
+    const int32_t p_last = before + static_cast<int32_t>(A.group.div(r1 - 1));
+    const uint32_t row = r0 + c < r1 ? r0 + c : r1 - 1, token = A.group.div(row), head = kvh * G + row - token * G;
+    const int32_t p = before + static_cast<int32_t>(token);
+    const int32_t window = static_cast<int32_t>(A.window & 0x7fffffffu); // (unbounded: 0, see below)
+    const bool bounded = A.window != 0x80000000u;
+    const int32_t from = bounded ? p - window + 1 : 0; // first position row c sees
+    const int32_t lo = bounded && p_first - window + 1 > 0 ? p_first - window + 1 : 0;
+    const int32_t hi = p_last + 1 > 0 ? p_last + 1 : 0;
+    // every row of the tile sees these
+    const int32_t all_lo = bounded ? p_last - window + 1 : 0, all_hi = p_first + 1;
+
+    Tile tile;
+    tile.load_q(A.q + (seq.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), g, D);
+#pragma unroll
+    for (int m = 0; m < Tile::kE; ++m) tile.acc[m] = f32x4{};
+    float top = kNegInf, mass = 0.0f;
+    const uint8_t *kp = a.k + kvh * a.head_bytes, *vp = a.v + kvh * a.head_bytes;
+    const uint32_t *table = a.table + static_cast<uint64_t>(index) * a.table_stride;
+    for (int32_t base = lo + static_cast<int32_t>(wave) * Tile::kKeys; base < hi; base += kWaves * Tile::kKeys) {
+        const int32_t mine = base + static_cast<int32_t>(lane & (Tile::kKeys - 1));
+        const uint32_t t = mine < hi ? mine : hi - 1; // reads stay in the sequence
+        const uint32_t page = a.page.div(t);
+        __builtin_amdgcn_wave_barrier();
+        offsets[wave][lane & (Tile::kKeys - 1)] = position_offset(a, table[page], t - page * a.page.d, bad);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        tile.load(kp, vp, offsets[wave], c, g, D);
+        float s[Tile::kScores];
+        tile.scores(s);
+        if (base + Tile::kKeys > hi) tile.clear_values(g, hi - base);
+        float high = kNegInf;
+        if (base >= all_lo && base + Tile::kKeys <= all_hi) {
+#pragma unroll
+            for (int x = 0; x < Tile::kScores; ++x) {
+                s[x] = log2_score(A, s[x]);
+                high = fmaxf(high, s[x]);
+            }
+        } else {
+            bool seen[Tile::kScores];
+#pragma unroll
+            for (int x = 0; x < Tile::kScores; ++x) {
+                const int32_t j = base + static_cast<int32_t>(Tile::key(g, x));
+                seen[x] = j <= p && j >= from;
+                s[x] = seen[x] ? log2_score(A, s[x]) : kNegInf;
+                high = fmaxf(high, s[x]);
+            }
+            tile.split_nonfinite(seen);
+        }
+        high = row_max(high);
+        const float next = fmaxf(top, high), at = next == kNegInf ? 0.0f : next;
+        const float shrink = exp2_fast(top - at);
+        float w[Tile::kScores], sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < Tile::kScores; ++x) {
+            w[x] = exp2_fast(s[x] - at + kLift);
+            sum += w[x];
+        }
+        top = next;
+        mass = mass * shrink + sum; // this lane's keys
+        if (__any(shrink != 1.0f))
+#pragma unroll
+            for (int m = 0; m < Tile::kE; ++m) tile.acc[m] *= shrink;
+        tile.template add<kParts>(w);
+    }
+    if (__any(bad) && lane == 0) atomicOr(A.status, STATUS_BAD_PAGE);
+    mass = row_sum(mass);
+    if (g == 0) {
+        top_s[wave][c] = top;
+        mass_s[wave][c] = mass;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int m = 0; m < Tile::kE; m += 4)
+            *reinterpret_cast<f32x4 *>(sums + (wave * kRows + c) * kStride + Tile::kE * (4 * g + i) + m) =
+                f32x4{tile.acc[m][i], tile.acc[m + 1][i], tile.acc[m + 2][i], tile.acc[m + 3][i]};
+    __syncthreads();
+    for (uint32_t u = tid; u < kRows * DP / 4; u += kThreads) {
+        const uint32_t r = u / (DP / 4), d = u % (DP / 4) * 4;
+        if (r0 + r >= r1 || d >= D) continue;
+        const uint32_t tok = A.group.div(r0 + r), h = kvh * G + r0 + r - tok * G;
+        float best = kNegInf;
+#pragma unroll
+        for (uint32_t i = 0; i < kWaves; ++i) best = fmaxf(best, top_s[i][r]);
+        float sink = kNegInf;
+        if (A.sinks) {
+            sink = A.sinks[h] * 0x1.715476p+0f; // log2 e
+            best = best == kNegInf ? best : fmaxf(best, sink);
+        }
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        float total = 0.0f;
+        if (best != kNegInf) {
+            if (A.sinks) total = exp2_fast(sink - best + kLift);
+#pragma unroll
+            for (uint32_t i = 0; i < kWaves; ++i) {
+                const float f = exp2_fast(top_s[i][r] - best);
+                total += f * mass_s[i][r];
+                o += f * *reinterpret_cast<const f32x4 *>(sums + (i * kRows + r) * kStride + d);
+            }
+            o /= total;
+        }
+        store4(A.out + (seq.start + tok) * A.out_bytes + static_cast<uint64_t>(h) * D * (A.out_type == FMX_TYPE_F32 ? 4 : 2),
+               d, A.out_type, o);
+    }
+}
+
+template <typename T, int DP, int kParts> int launch_rows(const AttentionArgs &A, hipStream_t s) {
+    const uint32_t G = A.group.d;
+    const uint64_t tiles = static_cast<uint64_t>(A.a.tokens) * G / kRows + A.a.sequences;
+    const uint64_t blocks = tiles * A.a.kv_heads;
+    if (blocks > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
+    const size_t lds = kWaves * kRows * (DP + 4) * sizeof(float);
+    const auto kernel = attention_rows_kernel<T, DP, kParts>;
+    if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), lds, s, A);
+    FMX_LAUNCH_CHECK();
+    return FMX_OK;
+}
+
+template <typename T, int kParts> int launch_dim(const AttentionArgs &A, hipStream_t s) {
+    if (A.a.head_dim <= 64) return launch_rows<T, 64, kParts>(A, s);
+    if (A.a.head_dim <= 128) return launch_rows<T, 128, kParts>(A, s);
+    return launch_rows<T, 256, kParts>(A, s);
+}
+
+template <typename T> int launch_type(const AttentionArgs &A, hipStream_t s) {
+    return A.out_type == FMX_TYPE_F32 ? launch_dim<T, Element<T>::kParts>(A, s) : launch_dim<T, 1>(A, s);
+}
+
+} // namespace
+
+uint64_t attention_paged_scratch(const PagedArgs &, uint32_t, uint32_t) { return 0; }
+
+int attention_paged(const PagedArgs &a, uint32_t type, const AttentionCall &c, hipStream_t s) {
+    AttentionArgs A;
+    A.a = a;
+    A.q = static_cast<const uint8_t *>(c.q);
+    A.out = static_cast<uint8_t *>(c.out);
+    A.q_bytes = c.q_stride * element_bytes(type);
+    A.out_bytes = c.out_stride * element_bytes(c.out_type);
+    A.heads = c.heads;
+    A.group = FastDiv(c.heads / a.kv_heads);
+    constexpr double kLog2e = 1.4426950408889634;
+    const double cap = c.options.softcap;
+    A.scale = static_cast<float>(cap != 0.0 ? c.options.scale / cap : c.options.scale * kLog2e);
+    A.softcap = static_cast<float>(cap * kLog2e);
+    A.window = c.options.window == 0 || c.options.window > 0x7fffffffu ? 0x80000000u : c.options.window;
+    A.sinks = c.options.sinks;
+    A.out_type = c.out_type;
+    A.status = c.status;
+    if (type == FMX_TYPE_F32) return launch_dim<float, 1>(A, s);
+    if (type == FMX_TYPE_F16) return launch_type<_Float16>(A, s);
+    return launch_type<__bf16>(A, s);
+}
+
+} // namespace fmx

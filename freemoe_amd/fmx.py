@@ -16,6 +16,9 @@ from pathlib import Path
 LIB_PATH = Path(os.environ.get("FMX_LIBRARY") or Path(__file__).resolve().parent / "libfmx.so")
 
 FMX_TYPE_F32, FMX_TYPE_Q4_0, FMX_TYPE_Q8_0, FMX_TYPE_Q4_K, FMX_TYPE_Q6_K = 0, 2, 8, 12, 14
+FMX_TYPE_F16, FMX_TYPE_BF16 = 1, 30
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN, ROPE_SCALE_BANDS = range(4)
 BLOCK_GEOMETRY = {FMX_TYPE_F32: (1, 4), FMX_TYPE_Q4_0: (32, 18), FMX_TYPE_Q8_0: (32, 34),
                   FMX_TYPE_Q4_K: (256, 144), FMX_TYPE_Q6_K: (256, 210)}
 FAULT_NONE, FAULT_TRANSFER, FAULT_FENCE_DEFERRED, FAULT_FENCE_TIMEOUT, FAULT_DEVICE_LOSS = range(5)
@@ -46,6 +49,41 @@ class MoELayer(ctypes.Structure):
                 ("weights_norm", c_int32), ("epsilon_additive", c_int32), ("weights_epsilon", c_double),
                 ("weights_scale", c_double), ("gate_type", c_uint32), ("up_type", c_uint32),
                 ("down_type", c_uint32), ("gate", c_void_p), ("up", c_void_p), ("down", c_void_p)]
+
+
+class PagedCache(ctypes.Structure):
+    """fmx_paged_cache: one layer's pages (device addresses, strides in elements)."""
+    _fields_ = [("type", c_uint32), ("kv_heads", c_uint32), ("head_dim", c_uint32), ("page_size", c_uint32),
+                ("pages", c_uint32), ("page_stride", c_uint64), ("position_stride", c_uint64),
+                ("head_stride", c_uint64), ("k", c_void_p), ("v", c_void_p)]
+
+
+class PagedBatch(ctypes.Structure):
+    """fmx_paged_batch: the sequences of a step (device arrays of uint32)."""
+    _fields_ = [("sequences", c_uint32), ("tokens", c_uint32), ("max_new", c_uint32), ("table_stride", c_uint32),
+                ("starts", c_void_p), ("lengths", c_void_p), ("table", c_void_p)]
+
+
+class RopeScaling(ctypes.Structure):
+    """fmx_rope_scaling."""
+    _fields_ = [("kind", c_uint32), ("base", c_double), ("factor", c_double), ("context", c_double),
+                ("low", c_double), ("high", c_double)]
+
+
+class Rope(ctypes.Structure):
+    """fmx_rope."""
+    _fields_ = [("layout", c_uint32), ("dims", c_uint32), ("inv_freq", c_void_p), ("magnitude", c_double),
+                ("positions", c_void_p)]
+
+
+class AttentionOptions(ctypes.Structure):
+    """fmx_attention_options."""
+    _fields_ = [("scale", c_double), ("softcap", c_double), ("window", c_uint32), ("sinks", c_void_p)]
+
+
+class Sampling(ctypes.Structure):
+    """fmx_sampling: per-row device arrays, None for the neutral value."""
+    _fields_ = [("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p), ("min_p", c_void_p)]
 
 
 _SIGNATURES = {
@@ -89,6 +127,16 @@ _SIGNATURES = {
     "fmx_moe_status_of": (c_int, [c_uint32]),
     "fmx_attention_decode": (c_int, [c_void_p, c_void_p, c_uint64, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32,
                                      c_double, c_void_p, c_void_p, c_uint64, c_void_p]),
+    "fmx_rope_frequencies": (c_int, [POINTER(RopeScaling), c_uint32, POINTER(c_double), POINTER(c_double)]),
+    "fmx_rope_append": (c_int, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rope), c_uint32, c_uint32, c_void_p,
+                                c_uint64, c_void_p, c_uint64, c_void_p, c_uint64, c_void_p, c_uint64, c_void_p,
+                                c_uint64, c_void_p]),
+    "fmx_attention_paged_workspace_bytes": (c_uint64, [POINTER(PagedCache), POINTER(PagedBatch), c_uint32]),
+    "fmx_attention_paged": (c_int, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(AttentionOptions), c_uint32,
+                                    c_void_p, c_uint64, c_uint32, c_void_p, c_uint64, c_void_p, c_uint64, c_void_p]),
+    "fmx_sample_workspace_bytes": (c_uint64, [c_uint32, c_uint32]),
+    "fmx_sample": (c_int, [c_void_p, c_uint64, c_uint32, c_uint32, POINTER(Sampling), c_void_p, c_void_p, c_void_p,
+                           c_void_p, c_uint64, c_void_p]),
     "fmx_moe_bucket": (c_int, [c_void_p, c_uint32, c_uint32, c_uint32, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_uint64, c_void_p]),
 }

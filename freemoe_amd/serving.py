@@ -1,0 +1,132 @@
+"""The serving operators driven through libfmx on torch tensors: a paged cache
+in HBM, rotary positions with the cache write, attention over the pages, and
+sampling.
+
+torch provides the device memory and the stream; every computation is a
+libfmx call. Sequences, their lengths and their pages are the caller's: a
+Batch holds the device arrays that name them, and a captured graph follows
+what those hold at each replay.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import fmx
+
+TYPE_IDS = {torch.float32: fmx.FMX_TYPE_F32, torch.float16: fmx.FMX_TYPE_F16, torch.bfloat16: fmx.FMX_TYPE_BF16}
+
+
+class Cache:
+    """One layer's keys and values: `pages` pages of `page_size` positions."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16, device="cuda"):
+        self.k = torch.zeros(pages, page_size, kv_heads, head_dim, dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.describe()
+
+    @classmethod
+    def of(cls, k: torch.Tensor, v: torch.Tensor) -> "Cache":
+        """On existing pools, [page, place, kv head, element] with any strides the library takes."""
+        if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.dim() != 4 or k.stride(3) != 1:
+            raise ValueError("k and v: alike, [page, place, kv head, element], elements next to each other")
+        self = cls.__new__(cls)
+        self.k, self.v = k, v
+        self.describe()
+        return self
+
+    def describe(self):
+        pages, page_size, kv_heads, head_dim = self.k.shape
+        # (torch gives dimensions of one entry any stride)
+        strides = [s if n > 1 else self.k.numel() for s, n in zip(self.k.stride(), self.k.shape)]
+        strides = [-(-max(s, head_dim) // 8) * 8 if n == 1 else s for s, n in zip(strides, self.k.shape)]
+        self.desc = fmx.PagedCache(TYPE_IDS[self.k.dtype], kv_heads, head_dim, page_size, pages, strides[0], strides[1],
+                                   strides[2], self.k.data_ptr(), self.v.data_ptr())
+
+
+class Batch:
+    """The new tokens of a step: starts [sequences + 1], lengths [sequences] and
+    table [sequences, pages of the longest], int32 on the device."""
+
+    def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, tokens: int, max_new: int):
+        for t in (starts, lengths, table):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError("starts, lengths and table: contiguous int32")
+        if starts.numel() != lengths.numel() + 1 or table.shape[0] != lengths.numel():
+            raise ValueError("starts: one more than lengths; table: a row per sequence")
+        self.starts, self.lengths, self.table, self.tokens = starts, lengths, table, tokens
+        self.desc = fmx.PagedBatch(lengths.numel(), tokens, max_new, table.shape[1], starts.data_ptr(),
+                                   lengths.data_ptr(), table.data_ptr())
+
+
+class Rope:
+    """The angles of a model: made once on the host, kept on the device."""
+
+    def __init__(self, dims: int, base: float = 10000.0, layout: int = fmx.ROPE_HALF, kind: int = fmx.ROPE_SCALE_NONE,
+                 factor: float = 1.0, context: float = 0.0, low: float = 1.0, high: float = 32.0, device="cuda"):
+        scaling = fmx.RopeScaling(kind, base, factor, context, low, high)
+        inv, magnitude = (ctypes.c_double * (dims // 2))(), ctypes.c_double()
+        fmx.call("fmx_rope_frequencies", ctypes.byref(scaling), dims, inv, ctypes.byref(magnitude))
+        self.inv_freq = torch.tensor(list(inv), dtype=torch.float64, device=device)
+        self.layout, self.dims, self.magnitude = layout, dims, magnitude.value
+
+    def desc(self, positions=None):
+        return fmx.Rope(self.layout, self.dims, self.inv_freq.data_ptr(), self.magnitude, fmx.ptr(positions) or None)
+
+
+def _rows(t: torch.Tensor, tokens: int) -> int:
+    """Row stride of [tokens, heads, head_dim] (the heads of a row next to each other)."""
+    if t.dim() != 3 or t.shape[0] < tokens or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError("rows: [tokens, heads, head_dim], a row's heads next to each other")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+
+
+def workspace(bytes_: int = 256, device="cuda") -> torch.Tensor:
+    return torch.zeros(bytes_, dtype=torch.uint8, device=device)
+
+
+def status(ws: torch.Tensor, stream=None) -> int:
+    """The error word's status; clears it. Waits for the stream."""
+    return fmx.lib().fmx_moe_status(ws.data_ptr(), fmx.stream_handle(stream))
+
+
+def rope_append(cache: Cache, batch: Batch, rope: Rope, q, k, v, q_out, ws, positions=None, stream=None):
+    fmx.call("fmx_rope_append", ctypes.byref(cache.desc), ctypes.byref(batch.desc), ctypes.byref(rope.desc(positions)),
+             q.shape[1], TYPE_IDS[q.dtype], q.data_ptr(), _rows(q, batch.tokens), k.data_ptr(), _rows(k, batch.tokens),
+             v.data_ptr(), _rows(v, batch.tokens), q_out.data_ptr(), _rows(q_out, batch.tokens), ws.data_ptr(),
+             ws.numel(), fmx.stream_handle(stream))
+    return q_out
+
+
+def attention_workspace(cache: Cache, batch: Batch, heads: int) -> torch.Tensor:
+    need = fmx.lib().fmx_attention_paged_workspace_bytes(ctypes.byref(cache.desc), ctypes.byref(batch.desc), heads)
+    if need == 0:
+        raise fmx.FmxError(1, "fmx_attention_paged_workspace_bytes")
+    return workspace(need, cache.k.device)
+
+
+def attention(cache: Cache, batch: Batch, q, out, ws, scale=None, softcap=0.0, window=0, sinks=None, stream=None):
+    options = fmx.AttentionOptions(1.0 / math.sqrt(q.shape[2]) if scale is None else scale, softcap, window,
+                                   fmx.ptr(sinks) or None)
+    fmx.call("fmx_attention_paged", ctypes.byref(cache.desc), ctypes.byref(batch.desc), ctypes.byref(options), q.shape[1],
+             q.data_ptr(), _rows(q, batch.tokens), TYPE_IDS[out.dtype], out.data_ptr(), _rows(out, batch.tokens),
+             ws.data_ptr(), ws.numel(), fmx.stream_handle(stream))
+    return out
+
+
+def sample(logits, uniform, ws=None, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, probs=None,
+           stream=None):
+    """Token ids (int32) and their probabilities, one per row of logits."""
+    rows, vocab = logits.shape
+    if logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise ValueError("logits: float32 rows")
+    ids = torch.empty(rows, dtype=torch.int32, device=logits.device) if ids is None else ids
+    probs = torch.empty(rows, dtype=torch.float32, device=logits.device) if probs is None else probs
+    ws = workspace(fmx.lib().fmx_sample_workspace_bytes(rows, vocab), logits.device) if ws is None else ws
+    settings = fmx.Sampling(*(fmx.ptr(t) or None for t in (temperature, top_k, top_p, min_p)))
+    fmx.call("fmx_sample", logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
+             ctypes.byref(settings), uniform.data_ptr(), ids.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(),
+             fmx.stream_handle(stream))
+    return ids, probs

@@ -57,6 +57,8 @@ typedef enum fmx_status {
 
 /* Tensor type ids (GGUF, gguf.cpp:58-106) this library executes. */
 enum { FMX_TYPE_F32 = 0, FMX_TYPE_Q4_0 = 2, FMX_TYPE_Q8_0 = 8, FMX_TYPE_Q4_K = 12, FMX_TYPE_Q6_K = 14 };
+/* Element types of paged caches and of the rows that go with them, besides F32. */
+enum { FMX_TYPE_F16 = 1, FMX_TYPE_BF16 = 30 };
 
 /* Faults forced from the host, as fm::BackendFault (include/fm/backend.hpp:118). */
 enum { FMX_FAULT_NONE = 0, FMX_FAULT_TRANSFER = 1, FMX_FAULT_FENCE_DEFERRED = 2,
@@ -294,6 +296,154 @@ int fmx_moe_bucket(const uint32_t *ids, uint32_t tokens, uint32_t top_k, uint32_
 int fmx_attention_decode(const float *q, const float *kv, uint64_t row_stride, uint32_t v_offset,
                          uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t positions,
                          double scale, float *out, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* ----------------------------------------------------------- paged cache -- */
+
+/* One layer's keys and values in pages: element d of kv head h at place i of
+ * page p lies at k (or v) + p * page_stride + i * position_stride +
+ * h * head_stride + d, strides in elements, so [page][place][head][d] and
+ * [page][head][place][d] pools and slices of larger ones are all taken.
+ * Strides are multiples of 16 bytes, k and v 16-byte aligned; offsets are
+ * formed in 64 bits. */
+typedef struct fmx_paged_cache {
+    uint32_t type;       /* FMX_TYPE_F32, FMX_TYPE_F16 or FMX_TYPE_BF16 */
+    uint32_t kv_heads;
+    uint32_t head_dim;   /* a multiple of 8, at most 256 */
+    uint32_t page_size;  /* positions of a page, any number from 1 to 65536 */
+    uint32_t pages;      /* in the pool: every table entry in use is below it */
+    uint64_t page_stride, position_stride, head_stride;
+    void *k, *v;
+} fmx_paged_cache;
+
+/* A ragged batch. Sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1
+ * of q, k, v and out; they are the last ones of its lengths[i] positions, and its
+ * position t is place t % page_size of page table[i * table_stride + t / page_size].
+ * starts ([sequences + 1], rising), lengths and table are device arrays, so a
+ * captured call follows what they hold at each replay; tokens, max_new and
+ * table_stride bound them from the host:
+ *   starts[sequences] <= tokens; rows behind it are neither read nor written
+ *   starts[i + 1] - starts[i] <= max_new
+ *   lengths[i] <= table_stride * page_size (itself below 2^31)
+ * An entry that breaks a bound or a page that is not in the pool is not
+ * followed: the kernels set a bit that fmx_moe_status reports as
+ * FMX_ERR_INVALID_ARGUMENT, and that sequence's results are not meaningful.
+ * Entries of the table behind a sequence's last page are not read. Sequences
+ * may share pages that none of them writes. */
+typedef struct fmx_paged_batch {
+    uint32_t sequences;
+    uint32_t tokens;
+    uint32_t max_new;
+    uint32_t table_stride;
+    const uint32_t *starts;
+    const uint32_t *lengths;
+    const uint32_t *table;
+} fmx_paged_batch;
+
+/* The error word of the calls below is the first of their workspace, as for
+ * the MoE calls, but they only add to it: zeroed with the workspace (fmx_alloc
+ * does) and by fmx_moe_status, it holds what any call since then met, so a
+ * program reads it once per step. A workspace serves one call at a time. */
+
+/* Rotary positions. */
+enum { FMX_ROPE_INTERLEAVED = 0,  /* pairs (2c, 2c + 1) */
+       FMX_ROPE_HALF = 1 };       /* pairs (c, c + dims / 2) */
+
+/* How the angles are stretched to contexts longer than the trained one. */
+enum { FMX_ROPE_SCALE_NONE = 0,
+       FMX_ROPE_SCALE_LINEAR = 1,  /* every position divided by factor */
+       FMX_ROPE_SCALE_YARN = 2,    /* by pair: fast ones kept, slow ones divided, a ramp between */
+       FMX_ROPE_SCALE_BANDS = 3 }; /* by wavelength: below context / high kept, above context / low
+                                      divided, blended between */
+
+typedef struct fmx_rope_scaling {
+    uint32_t kind;
+    double base;         /* 10000 and the like */
+    double factor;       /* >= 1 */
+    double context;      /* the positions the angles were trained for */
+    double low, high;    /* yarn: turns over the context at which a pair is slow / fast (1, 32);
+                            bands: low and high frequency factor (1, 4) */
+} fmx_rope_scaling;
+
+/* The angle per position of each of dims / 2 pairs and the magnitude that goes
+ * with them (yarn: 0.1 ln factor + 1, else 1). Host arrays, host arithmetic in
+ * double; a program uploads inv_freq once per model. */
+int fmx_rope_frequencies(const fmx_rope_scaling *scaling, uint32_t dims, double *inv_freq, double *magnitude);
+
+typedef struct fmx_rope {
+    uint32_t layout;          /* FMX_ROPE_* */
+    uint32_t dims;            /* first elements of each head that turn: even, at most head_dim */
+    const double *inv_freq;   /* device [dims / 2], radians per position */
+    double magnitude;         /* of cos and sin */
+    const int32_t *positions; /* device [tokens] positions of the angles, NULL: those in the cache */
+} fmx_rope;
+
+/* Rotates q and k and writes k and v into the batch's pages: the rows of q
+ * ([heads x head_dim] each, q_stride elements apart), k and v ([kv_heads x
+ * head_dim]) of in_type (FMX_TYPE_F32 or the cache's type) become q_out's rows
+ * of the cache's type, and the cache's. Angles are formed and reduced in
+ * double, pairs turned in f32, each result rounded once; elements from dims on
+ * are copied. q_out may be q where types and strides agree. Strides are
+ * multiples of 16 bytes, pointers 16-byte aligned. workspace: >= 256 bytes,
+ * the error word (also set, and the token skipped, where a sequence has more
+ * new tokens than positions). */
+int fmx_rope_append(const fmx_paged_cache *cache, const fmx_paged_batch *batch, const fmx_rope *rope,
+                    uint32_t heads, uint32_t in_type, const void *q, uint64_t q_stride, const void *k,
+                    uint64_t k_stride, const void *v, uint64_t v_stride, void *q_out, uint64_t q_out_stride,
+                    void *workspace, uint64_t workspace_bytes, void *stream);
+
+typedef struct fmx_attention_options {
+    double scale;        /* of q . k; 1 / sqrt(head_dim) as a rule */
+    double softcap;      /* c > 0: scores become c tanh(score / c); 0: as they are */
+    uint32_t window;     /* positions a token sees, its own the last; 0: all before it */
+    const float *sinks;  /* device [heads] logits that join each head's softmax without a value, or NULL */
+} fmx_attention_options;
+
+/* Attention of the batch's new tokens over their sequences' pages, their own
+ * positions included (fmx_rope_append has written them): the token at position
+ * p sees positions max(0, p - window + 1) .. p of its sequence, query head h
+ * kv head h / (heads / kv_heads). q: rows [heads x head_dim] of the cache's type,
+ * q_stride elements apart; out: rows of out_type (FMX_TYPE_F32 or the cache's
+ * type), out_stride apart. Strides are multiples of 16 bytes, pointers 16-byte
+ * aligned. A token that sees nothing (more new tokens than positions) gets
+ * zeros. What a token does not see does not reach it, NaN and infinities there
+ * included; of those it does see, a score makes its row NaN and an element of a
+ * value that element of its row not finite. Scores and softmax statistics are
+ * f32. An f32 result carries f32 accuracy whatever the cache's
+ * type; for a 16-bit one the weights are rounded to 16 bits before they meet
+ * the values. max_new chooses the kernel: state it as it is. */
+uint64_t fmx_attention_paged_workspace_bytes(const fmx_paged_cache *cache, const fmx_paged_batch *batch,
+                                             uint32_t heads);
+int fmx_attention_paged(const fmx_paged_cache *cache, const fmx_paged_batch *batch,
+                        const fmx_attention_options *options, uint32_t heads, const void *q, uint64_t q_stride,
+                        uint32_t out_type, void *out, uint64_t out_stride, void *workspace,
+                        uint64_t workspace_bytes, void *stream);
+
+/* -------------------------------------------------------------- sampling -- */
+
+/* Per-row settings, device arrays of one entry per row; NULL: the neutral value. */
+typedef struct fmx_sampling {
+    const float *temperature; /* 0: the largest logit, 1 where NULL */
+    const uint32_t *top_k;    /* 0 or NULL: all */
+    const float *top_p;       /* >= 1 or NULL: all */
+    const float *min_p;       /* <= 0 or NULL: all */
+} fmx_sampling;
+
+/* One token per row of logits ([rows x vocab], row_stride elements apart),
+ * from one uniform number in [0, 1) each. Tokens are ordered by falling logit,
+ * equal ones by rising id, and weighted w = exp((logit - largest) / temperature);
+ * kept are the first top_k, of these the shortest prefix that holds top_p of
+ * their mass, and of these the ones with w >= min_p (at least one); ids[row] is
+ * the first whose cumulated mass exceeds uniform x the mass kept, probs[row]
+ * (may be NULL) its share of that mass. Masses are sums of w in 2^-44 steps,
+ * the same in whatever order they are added, so a row's token depends on
+ * nothing but its inputs. Logits of -inf are never chosen. A row with a NaN or
+ * +inf or without a finite logit, a temperature below 0 or a NaN setting gives
+ * ids[row] = 0xffffffff, probs[row] = 0 and FMX_ERR_INTERNAL from
+ * fmx_moe_status. vocab <= 262144. */
+uint64_t fmx_sample_workspace_bytes(uint32_t rows, uint32_t vocab);
+int fmx_sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
+               const fmx_sampling *sampling, const float *uniform, uint32_t *ids, float *probs,
+               void *workspace, uint64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
