@@ -100,6 +100,14 @@ __device__ __forceinline__ bool find_item(const PagedArgs &a, uint32_t target, c
     return false;
 }
 
+// Whether any sequence breaks a bound: for one workgroup of a call, since those
+// behind the last item a wavefront looks for are not passed on its way.
+__device__ __forceinline__ bool any_bad_sequence(const PagedArgs &a) {
+    bool bad = false;
+    for (uint32_t i = threadIdx.x & 63; i < a.sequences; i += 64) bad |= sequence_at(a, i).bad;
+    return __any(bad);
+}
+
 // rope.hip, paged_attention.hip, sample.hip: the entry points after their
 // pointer checks.
 struct RopeCall {

@@ -22,6 +22,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
+constexpr uint32_t kUnbounded = 0x80000000u; // a window: all positions before
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kThreads = 64 * kWaves;
 
@@ -34,11 +35,75 @@ struct AttentionArgs {
     FastDiv group;               // query heads of a kv head
     float scale;                 // times log2 e (softcap: 1 / softcap times the plain one)
     float softcap;               // times log2 e, or 0
-    uint32_t window;             // 0x80000000 where there is none
+    uint32_t window;             // or kUnbounded
     const float *sinks;
     uint32_t out_type;
     uint32_t *status;
+    // splits > 1: a tile's keys go to that many workgroups at most, whose sums
+    // meet in `parts` and `stats` (below)
+    uint32_t splits;
+    float *parts;  // [tile][kv head][split][row][head_dim]
+    float2 *stats; // [tile][kv head][split][row]: maximum, sum
 };
+
+// What one workgroup has of a tile of rows: its sequence, rows and keys.
+struct Job {
+    uint32_t index, start, r0, r1, kvh, slot; // slot: of its sums, where they are split
+    int32_t before;                           // position of the sequence's first new token
+    int32_t lo, hi;                           // this workgroup's keys
+    bool whole;                               // all of the tile's keys are its
+};
+
+// The keys of a tile go out in equal pieces of whole `unit`s; the pieces that
+// hold any number `pieces`.
+struct Pieces {
+    uint32_t size, count;
+};
+__device__ __forceinline__ Pieces pieces_of(uint32_t keys, uint32_t splits, uint32_t unit) {
+    const uint32_t units = (keys + unit - 1) / unit, each = (units + splits - 1) / splits;
+    return Pieces{each * unit, each ? (units + each - 1) / each : 0};
+}
+
+// The visible keys of rows r0 .. r1 - 1: [lo, hi).
+__device__ __forceinline__ void visible_keys(const AttentionArgs &A, int32_t before, uint32_t r0, uint32_t r1,
+                                             int32_t &lo, int32_t &hi) {
+    const int32_t first = before + static_cast<int32_t>(A.group.div(r0));
+    hi = before + static_cast<int32_t>(A.group.div(r1 - 1)) + 1;
+    hi = hi > 0 ? hi : 0;
+    lo = A.window != kUnbounded && first - static_cast<int32_t>(A.window) + 1 > 0
+             ? first - static_cast<int32_t>(A.window) + 1 : 0;
+    lo &= ~3; // groups of four keys share a page where the page size allows
+}
+
+// Workgroup -> job: splits slowest (so that a tile's workgroups are spread over
+// time as little as over the chip), kv heads fastest.
+template <uint32_t kTileRows, uint32_t kUnit>
+__device__ __forceinline__ bool find_job(const AttentionArgs &A, uint32_t block, Job &job, bool &bad) {
+    const PagedArgs &a = A.a;
+    const uint32_t G = A.group.d;
+    job.kvh = block % a.kv_heads;
+    const uint32_t rest = block / a.kv_heads, split = rest % A.splits, target = rest / A.splits;
+    uint32_t item;
+    Sequence seq;
+    if (block == 0 && a.sequences > 64) bad |= any_bad_sequence(a);
+    if (!find_item(a, target, [&](const Sequence &s) { return (s.count * G + kTileRows - 1) / kTileRows; }, job.index,
+                   seq, item, bad))
+        return false;
+    const uint32_t rows = seq.count * G;
+    job.start = seq.start;
+    job.r0 = item * kTileRows;
+    job.r1 = job.r0 + kTileRows < rows ? job.r0 + kTileRows : rows;
+    job.before = static_cast<int32_t>(seq.length) - static_cast<int32_t>(seq.count);
+    job.slot = (target * a.kv_heads + job.kvh) * A.splits + split;
+    visible_keys(A, job.before, job.r0, job.r1, job.lo, job.hi);
+    const Pieces p = pieces_of(job.hi - job.lo, A.splits, kUnit);
+    job.whole = p.count <= 1;
+    if (split >= p.count) return split == 0; // (a tile without keys is split 0's)
+    job.lo += split * p.size;
+    const int32_t end = job.lo + static_cast<int32_t>(p.size);
+    job.hi = end < job.hi ? end : job.hi;
+    return true;
+}
 
 // Element types: how many 16-bit parts carry a weight to f32 accuracy, and the
 // power of two the weights are kept at. A half's range ends at 2^-24, which
@@ -318,11 +383,36 @@ __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, uint32_t type, 
     }
 }
 
+// Four elements of a row's sums with their maximum and the sum of weights: to
+// the output, with the sink's weight and divided, or, of a split tile, to where
+// attention_join_kernel takes them up.
+__device__ __forceinline__ void finish(const AttentionArgs &A, const Job &job, uint32_t tile_rows, uint32_t r,
+                                       uint32_t head, uint32_t token, uint32_t d, float top, float mass, f32x4 o,
+                                       float lift) {
+    const uint32_t D = A.a.head_dim;
+    if (!job.whole) {
+        const uint64_t at = static_cast<uint64_t>(job.slot) * tile_rows + r;
+        *reinterpret_cast<f32x4 *>(A.parts + at * D + d) = o;
+        if (d == 0) A.stats[at] = make_float2(top, mass);
+        return;
+    }
+    if (A.sinks && top != kNegInf) {
+        const float sink = A.sinks[head] * 0x1.715476p+0f; // log2 e
+        const float best = fmaxf(top, sink), f = exp2_fast(top - best);
+        mass = mass * f + exp2_fast(sink - best + lift);
+        o *= f;
+    }
+    if (top == kNegInf) o = f32x4{};
+    else o /= mass;
+    const uint32_t size = A.out_type == FMX_TYPE_F32 ? 4 : 2;
+    store4(A.out + token * A.out_bytes + static_cast<uint64_t>(head) * D * size, d, A.out_type, o);
+}
+
 constexpr uint32_t kRows = 16;
 
 // 16 rows of one sequence and kv head per workgroup; its wavefronts take tiles
 // of keys in turn and join their sums through LDS.
-// grid: row tiles x kv heads, the heads fastest.
+// grid: row tiles x splits x kv heads, the heads fastest.
 template <typename T, int DP, int kParts>
 __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs A) {
     using Tile = Tile16<T, DP>;
@@ -334,37 +424,32 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
     __shared__ float top_s[kWaves][kRows], mass_s[kWaves][kRows];
     const PagedArgs &a = A.a;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, target = blockIdx.x / a.kv_heads, G = A.group.d, D = a.head_dim;
-    uint32_t index, item;
-    Sequence seq;
+    const uint32_t G = A.group.d, D = a.head_dim;
     bool bad = false;
-    const bool found = find_item(
-        a, target, [&](const Sequence &s) { return (s.count * G + kRows - 1) / kRows; }, index, seq, item, bad);
-    if (!found) {
+    Job job;
+    if (!find_job<kRows, Tile::kKeys * kWaves>(A, blockIdx.x, job, bad)) {
         if (bad && tid == 0) atomicOr(A.status, STATUS_BAD_PAGE);
         return;
     }
-    const uint32_t rows = seq.count * G, r0 = item * kRows, r1 = r0 + kRows < rows ? r0 + kRows : rows;
-    const int32_t before = static_cast<int32_t>(seq.length) - static_cast<int32_t>(seq.count);
-    const int32_t p_first = before + static_cast<int32_t>(A.group.div(r0));
-    const int32_t p_last = before + static_cast<int32_t>(A.group.div(r1 - 1));
+    const uint32_t r0 = job.r0, r1 = job.r1, kvh = job.kvh;
+    const int32_t lo = job.lo, hi = job.hi;
+    const int32_t p_first = job.before + static_cast<int32_t>(A.group.div(r0));
+    const int32_t p_last = job.before + static_cast<int32_t>(A.group.div(r1 - 1));
     const uint32_t row = r0 + c < r1 ? r0 + c : r1 - 1, token = A.group.div(row), head = kvh * G + row - token * G;
-    const int32_t p = before + static_cast<int32_t>(token);
-    const int32_t window = static_cast<int32_t>(A.window & 0x7fffffffu); // (unbounded: 0, see below)
-    const bool bounded = A.window != 0x80000000u;
+    const int32_t p = job.before + static_cast<int32_t>(token);
+    const bool bounded = A.window != kUnbounded;
+    const int32_t window = static_cast<int32_t>(A.window);
     const int32_t from = bounded ? p - window + 1 : 0; // first position row c sees
-    const int32_t lo = bounded && p_first - window + 1 > 0 ? p_first - window + 1 : 0;
-    const int32_t hi = p_last + 1 > 0 ? p_last + 1 : 0;
     // every row of the tile sees these
     const int32_t all_lo = bounded ? p_last - window + 1 : 0, all_hi = p_first + 1;
 
     Tile tile;
-    tile.load_q(A.q + (seq.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), g, D);
+    tile.load_q(A.q + (job.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), g, D);
 #pragma unroll
     for (int m = 0; m < Tile::kE; ++m) tile.acc[m] = f32x4{};
     float top = kNegInf, mass = 0.0f;
     const uint8_t *kp = a.k + kvh * a.head_bytes, *vp = a.v + kvh * a.head_bytes;
-    const uint32_t *table = a.table + static_cast<uint64_t>(index) * a.table_stride;
+    const uint32_t *table = a.table + static_cast<uint64_t>(job.index) * a.table_stride;
     for (int32_t base = lo + static_cast<int32_t>(wave) * Tile::kKeys; base < hi; base += kWaves * Tile::kKeys) {
         const int32_t mine = base + static_cast<int32_t>(lane & (Tile::kKeys - 1));
         const uint32_t t = mine < hi ? mine : hi - 1; // reads stay in the sequence
@@ -432,54 +517,159 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
         float best = kNegInf;
 #pragma unroll
         for (uint32_t i = 0; i < kWaves; ++i) best = fmaxf(best, top_s[i][r]);
-        float sink = kNegInf;
-        if (A.sinks) {
-            sink = A.sinks[h] * 0x1.715476p+0f; // log2 e
-            best = best == kNegInf ? best : fmaxf(best, sink);
-        }
+        const float at = best == kNegInf ? 0.0f : best;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
         float total = 0.0f;
-        if (best != kNegInf) {
-            if (A.sinks) total = exp2_fast(sink - best + kLift);
 #pragma unroll
-            for (uint32_t i = 0; i < kWaves; ++i) {
-                const float f = exp2_fast(top_s[i][r] - best);
-                total += f * mass_s[i][r];
-                o += f * *reinterpret_cast<const f32x4 *>(sums + (i * kRows + r) * kStride + d);
-            }
-            o /= total;
+        for (uint32_t i = 0; i < kWaves; ++i) {
+            const float f = exp2_fast(top_s[i][r] - at);
+            total += f * mass_s[i][r];
+            o += f * *reinterpret_cast<const f32x4 *>(sums + (i * kRows + r) * kStride + d);
         }
-        store4(A.out + (seq.start + tok) * A.out_bytes + static_cast<uint64_t>(h) * D * (A.out_type == FMX_TYPE_F32 ? 4 : 2),
-               d, A.out_type, o);
+        finish(A, job, kRows, r, h, job.start + tok, d, best, total, o, kLift);
     }
 }
 
-template <typename T, int DP, int kParts> int launch_rows(const AttentionArgs &A, hipStream_t s) {
-    const uint32_t G = A.group.d;
-    const uint64_t tiles = static_cast<uint64_t>(A.a.tokens) * G / kRows + A.a.sequences;
-    const uint64_t blocks = tiles * A.a.kv_heads;
+// A split tile's sums joined: DP / 4 lanes hold a row of one head, kGroups such
+// groups take its pieces in turn. grid: row tiles x kv heads x workgroups of a
+// tile, these fastest.
+template <int DP, uint32_t kGroups>
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs A, uint32_t tile_rows, uint32_t unit,
+                                                                  float lift) {
+    constexpr uint32_t kLanes = DP / 4, kSlots = kThreads / kLanes, kRowsHere = kSlots / kGroups;
+    __shared__ f32x4 sum_s[kThreads];
+    __shared__ float2 stat_s[kSlots];
+    const PagedArgs &a = A.a;
+    const uint32_t G = A.group.d, D = a.head_dim, here = tile_rows / kRowsHere;
+    const uint32_t rest = blockIdx.x / here, kvh = rest % a.kv_heads, target = rest / a.kv_heads;
+    const uint32_t tid = threadIdx.x, d = tid % kLanes * 4, slot = tid / kLanes, group = slot % kGroups;
+    const uint32_t r = blockIdx.x % here * kRowsHere + slot / kGroups;
+    Job job;
+    uint32_t item;
+    Sequence seq;
+    bool bad = false; // (the tiles' own kernel reports it)
+    if (!find_item(a, target, [&](const Sequence &s) { return (s.count * G + tile_rows - 1) / tile_rows; }, job.index,
+                   seq, item, bad))
+        return;
+    const uint32_t rows = seq.count * G;
+    job.r0 = item * tile_rows;
+    job.r1 = job.r0 + tile_rows < rows ? job.r0 + tile_rows : rows;
+    job.before = static_cast<int32_t>(seq.length) - static_cast<int32_t>(seq.count);
+    visible_keys(A, job.before, job.r0, job.r1, job.lo, job.hi);
+    const uint32_t count = pieces_of(job.hi - job.lo, A.splits, unit).count;
+    if (count <= 1) return;
+    job.whole = true;
+    const bool mine = job.r0 + r < job.r1 && d < D;
+    const uint64_t first = static_cast<uint64_t>(target * a.kv_heads + kvh) * A.splits;
+    float top = kNegInf, mass = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine)
+#pragma unroll 4
+        for (uint32_t i = group; i < count; i += kGroups) {
+            const uint64_t at = (first + i) * tile_rows + r;
+            const float2 st = A.stats[at];
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(A.parts + at * D + d);
+            const float next = fmaxf(top, st.x), safe = next == kNegInf ? 0.0f : next;
+            const float f = exp2_fast(top - safe), g = exp2_fast(st.x - safe);
+            mass = mass * f + st.y * g;
+            o = o * f + x * g;
+            top = next;
+        }
+    if constexpr (kGroups > 1) {
+        sum_s[tid] = o;
+        if (d == 0) stat_s[slot] = make_float2(top, mass);
+        __syncthreads();
+        if (group != 0) return;
+        for (uint32_t i = 1; i < kGroups; ++i) {
+            const float2 st = stat_s[slot + i];
+            const f32x4 x = sum_s[tid + i * kLanes];
+            const float next = fmaxf(top, st.x), safe = next == kNegInf ? 0.0f : next;
+            const float f = exp2_fast(top - safe), g = exp2_fast(st.x - safe);
+            mass = mass * f + st.y * g;
+            o = o * f + x * g;
+            top = next;
+        }
+    }
+    if (!mine) return;
+    const uint32_t tok = A.group.div(job.r0 + r), head = kvh * G + job.r0 + r - tok * G;
+    finish(A, job, tile_rows, r, head, seq.start + tok, d, top, mass, o, lift);
+}
+
+// A split is worth its second launch and its sums' way through memory where
+// the tiles alone leave CUs idle; never into pieces below one unit of keys.
+constexpr uint32_t kFill = 2048; // workgroups that a split aims at
+
+// Scratch of a split call: stats, then sums.
+struct Scratch {
+    uint64_t stats, total;
+};
+Scratch scratch_of(uint64_t tiles, uint32_t kv_heads, uint32_t splits, uint32_t tile_rows, uint32_t head_dim) {
+    const uint64_t rows = tiles * kv_heads * splits * tile_rows;
+    const uint64_t stats = align_up(rows * sizeof(float2), 256);
+    return Scratch{stats, stats + align_up(rows * head_dim * sizeof(float), 256)};
+}
+
+uint64_t tiles_of(const PagedArgs &a, uint32_t group, uint32_t tile_rows) {
+    return static_cast<uint64_t>(a.tokens) * group / tile_rows + (a.sequences < a.tokens ? a.sequences : a.tokens);
+}
+
+uint32_t splits_of(const PagedArgs &a, uint64_t tiles, uint32_t unit) {
+    const uint64_t blocks = tiles * a.kv_heads;
+    const uint32_t most = div_up(a.max_length, unit);
+    const uint64_t want = (kFill + blocks - 1) / blocks;
+    return static_cast<uint32_t>(want < most ? want : most);
+}
+
+constexpr uint32_t rows_unit(uint32_t type) { return (type == FMX_TYPE_F32 ? 16 : 32) * kWaves; }
+
+template <typename T, int DP> int launch_join(const AttentionArgs &A, uint64_t tiles, uint32_t tile_rows, uint32_t unit,
+                                              hipStream_t s) {
+    if (A.splits <= 1) return FMX_OK;
+    constexpr uint32_t kSlots = kThreads / (DP / 4);
+    const bool many = A.splits > 8;
+    const uint64_t blocks = tiles * A.a.kv_heads * (tile_rows / (many ? 1 : kSlots));
+    if (blocks > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
+    const auto kernel = many ? attention_join_kernel<DP, kSlots> : attention_join_kernel<DP, 1>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, s, A, tile_rows, unit,
+                       Element<T>::kLift);
+    FMX_LAUNCH_CHECK();
+    return FMX_OK;
+}
+
+template <typename T, int DP, int kParts> int launch_rows(AttentionArgs A, uint8_t *scratch, uint32_t type, hipStream_t s) {
+    const uint64_t tiles = tiles_of(A.a, A.group.d, kRows);
+    const uint32_t unit = rows_unit(type);
+    A.splits = splits_of(A.a, tiles, unit);
+    A.stats = reinterpret_cast<float2 *>(scratch);
+    A.parts = reinterpret_cast<float *>(scratch + scratch_of(tiles, A.a.kv_heads, A.splits, kRows, A.a.head_dim).stats);
+    const uint64_t blocks = tiles * A.a.kv_heads * A.splits;
     if (blocks > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
     const size_t lds = kWaves * kRows * (DP + 4) * sizeof(float);
     const auto kernel = attention_rows_kernel<T, DP, kParts>;
     if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), lds, s, A);
     FMX_LAUNCH_CHECK();
-    return FMX_OK;
+    return launch_join<T, DP>(A, tiles, kRows, unit, s);
 }
 
-template <typename T, int kParts> int launch_dim(const AttentionArgs &A, hipStream_t s) {
-    if (A.a.head_dim <= 64) return launch_rows<T, 64, kParts>(A, s);
-    if (A.a.head_dim <= 128) return launch_rows<T, 128, kParts>(A, s);
-    return launch_rows<T, 256, kParts>(A, s);
+template <typename T, int kParts> int launch_dim(const AttentionArgs &A, uint8_t *scratch, uint32_t type, hipStream_t s) {
+    if (A.a.head_dim <= 64) return launch_rows<T, 64, kParts>(A, scratch, type, s);
+    if (A.a.head_dim <= 128) return launch_rows<T, 128, kParts>(A, scratch, type, s);
+    return launch_rows<T, 256, kParts>(A, scratch, type, s);
 }
 
-template <typename T> int launch_type(const AttentionArgs &A, hipStream_t s) {
-    return A.out_type == FMX_TYPE_F32 ? launch_dim<T, Element<T>::kParts>(A, s) : launch_dim<T, 1>(A, s);
+template <typename T> int launch_type(const AttentionArgs &A, uint8_t *scratch, uint32_t type, hipStream_t s) {
+    return A.out_type == FMX_TYPE_F32 ? launch_dim<T, Element<T>::kParts>(A, scratch, type, s)
+                                      : launch_dim<T, 1>(A, scratch, type, s);
 }
 
 } // namespace
 
-uint64_t attention_paged_scratch(const PagedArgs &, uint32_t, uint32_t) { return 0; }
+uint64_t attention_paged_scratch(const PagedArgs &a, uint32_t type, uint32_t heads) {
+    const uint64_t tiles = tiles_of(a, heads / a.kv_heads, kRows);
+    const uint32_t splits = splits_of(a, tiles, rows_unit(type));
+    return splits > 1 ? scratch_of(tiles, a.kv_heads, splits, kRows, a.head_dim).total : 0;
+}
 
 int attention_paged(const PagedArgs &a, uint32_t type, const AttentionCall &c, hipStream_t s) {
     AttentionArgs A;
@@ -494,13 +684,16 @@ int attention_paged(const PagedArgs &a, uint32_t type, const AttentionCall &c, h
     const double cap = c.options.softcap;
     A.scale = static_cast<float>(cap != 0.0 ? c.options.scale / cap : c.options.scale * kLog2e);
     A.softcap = static_cast<float>(cap * kLog2e);
-    A.window = c.options.window == 0 || c.options.window > 0x7fffffffu ? 0x80000000u : c.options.window;
+    A.window = c.options.window == 0 || c.options.window > 0x7fffffffu ? kUnbounded : c.options.window;
     A.sinks = c.options.sinks;
     A.out_type = c.out_type;
     A.status = c.status;
-    if (type == FMX_TYPE_F32) return launch_dim<float, 1>(A, s);
-    if (type == FMX_TYPE_F16) return launch_type<_Float16>(A, s);
-    return launch_type<__bf16>(A, s);
+    A.splits = 1;
+    A.parts = nullptr;
+    A.stats = nullptr;
+    if (type == FMX_TYPE_F32) return launch_dim<float, 1>(A, c.scratch, type, s);
+    if (type == FMX_TYPE_F16) return launch_type<_Float16>(A, c.scratch, type, s);
+    return launch_type<__bf16>(A, c.scratch, type, s);
 }
 
 } // namespace fmx

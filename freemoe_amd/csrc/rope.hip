@@ -73,6 +73,7 @@ __global__ __launch_bounds__(kThreads) void rope_append_kernel(PagedArgs a, Rope
     bool bad = false;
     const bool found =
         find_item(a, blockIdx.x, [](const Sequence &s) { return s.count; }, index, seq, item, bad);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && a.sequences > 64) bad |= any_bad_sequence(a);
     uint64_t at = 0;
     uint32_t row = 0;
     bool skip = !found;
