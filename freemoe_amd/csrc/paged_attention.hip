@@ -365,10 +365,13 @@ template <int DP> struct Tile16<float, DP> {
     }
 };
 
-// A score in units of log 2 from q . k.
-__device__ __forceinline__ float log2_score(const AttentionArgs &A, float dot) {
-    const float s = dot * A.scale;
-    return A.softcap != 0.0f ? tanhf(s) * A.softcap : s;
+// Scores in units of log 2 from q . k.
+template <int kN> __device__ __forceinline__ void log2_scores(const AttentionArgs &A, float *s) {
+#pragma unroll
+    for (int x = 0; x < kN; ++x) s[x] *= A.scale;
+    if (A.softcap != 0.0f)
+#pragma unroll
+        for (int x = 0; x < kN; ++x) s[x] = tanhf(s[x]) * A.softcap;
 }
 
 __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, uint32_t type, f32x4 x) {
@@ -463,24 +466,20 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
         float s[Tile::kScores];
         tile.scores(s);
         if (base + Tile::kKeys > hi) tile.clear_values(g, hi - base);
+        log2_scores<Tile::kScores>(A, s);
         float high = kNegInf;
-        if (base >= all_lo && base + Tile::kKeys <= all_hi) {
-#pragma unroll
-            for (int x = 0; x < Tile::kScores; ++x) {
-                s[x] = log2_score(A, s[x]);
-                high = fmaxf(high, s[x]);
-            }
-        } else {
+        if (base < all_lo || base + Tile::kKeys > all_hi) {
             bool seen[Tile::kScores];
 #pragma unroll
             for (int x = 0; x < Tile::kScores; ++x) {
                 const int32_t j = base + static_cast<int32_t>(Tile::key(g, x));
                 seen[x] = j <= p && j >= from;
-                s[x] = seen[x] ? log2_score(A, s[x]) : kNegInf;
-                high = fmaxf(high, s[x]);
+                s[x] = seen[x] ? s[x] : kNegInf;
             }
             tile.split_nonfinite(seen);
         }
+#pragma unroll
+        for (int x = 0; x < Tile::kScores; ++x) high = fmaxf(high, s[x]);
         high = row_max(high);
         const float next = fmaxf(top, high), at = next == kNegInf ? 0.0f : next;
         const float shrink = exp2_fast(top - at);
@@ -528,6 +527,366 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
         }
         finish(A, job, kRows, r, h, job.start + tok, d, best, total, o, kLift);
     }
+}
+
+// ------------------------------------------------------------ many rows --
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mma32(Vec8<__bf16>::type a, Vec8<__bf16>::type b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(Vec8<_Float16>::type a, Vec8<_Float16>::type b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// One wavefront's 32 rows against a tile of kKeys keys in LDS. The scores are
+// formed transposed as above: lane (c = lane % 32, h = lane / 32) holds row c's
+// scores, register 8 u + x of a 32-key block being key 16 u + 8 (x / 4) + 4 h +
+// x % 4, which as they stand are slots 8 h + x of the value product's step u.
+//
+// LDS holds keys and values as memory does, a row per position, its 16-byte
+// granules permuted so that every pass of a wavefront's reads touches all 64
+// banks: the key operand takes one granule of 16 consecutive rows, the value
+// operand (ds_read_b64_tr_b16: 16 lanes read 4 rows x 16 elements and each
+// gets one column) a 64-byte piece of 4 rows.
+template <typename T, int DP> struct Tile32 {
+    static constexpr int kKeys = DP == 256 ? 32 : 64, kBlocks = kKeys / 32, kSteps = DP / 16, kD = DP / 32;
+    static constexpr int kScores = 16 * kBlocks, kGranules = DP / 8, kGranule = 8;
+    static constexpr int kPerThread = kKeys * kGranules / kThreads; // consecutive keys a thread stages
+    typedef typename Vec8<T>::type v8;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    v8 q[kSteps];
+    f32x16 acc[kD];
+
+    static __device__ __forceinline__ uint32_t key_place(uint32_t key, uint32_t granule) {
+        return key * (DP * 2) + (granule ^ (DP == 64 ? key >> 1 & 7 : key & 15)) * 16;
+    }
+    static __device__ __forceinline__ uint32_t value_place(uint32_t key, uint32_t granule) {
+        return key * (DP * 2) + (granule ^ (DP == 64 ? (key >> 1 & 1) * 4 : (key & 3) * 4)) * 16;
+    }
+    static __device__ __forceinline__ uint32_t key(uint32_t h, int x) {
+        return x / 16 * 32 + x % 16 / 4 * 8 + 4 * h + x % 4;
+    }
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t h, uint32_t D) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] = v8{};
+            if (16 * s + 8 * h < D) q[s] = __builtin_bit_cast(v8, ld16(row + (16 * s + 8 * h) * 2));
+        }
+    }
+    __device__ __forceinline__ void scores(const char *keys, uint32_t c, uint32_t h, float *s) const {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            f32x16 r = {};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                r = mma32(*reinterpret_cast<const v8 *>(keys + key_place(32 * b + c, 2 * i + h)), q[i], r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[16 * b + i] = r[i];
+        }
+    }
+    // Value operand of block b, step u, elements 32 d .. 32 d + 31.
+    static __device__ __forceinline__ v8 value(const char *values, uint32_t lane, int b, int u, int d) {
+        typedef __attribute__((address_space(3))) s16x4 *ptr;
+        const uint32_t g = lane >> 4, i = lane & 15;
+        const uint32_t row = 32 * b + 16 * u + 4 * (g >> 1) + (i >> 2);
+        const uint32_t granule = 4 * d + 2 * (g & 1) + (i >> 1 & 1), byte = 8 * (i & 1);
+        const char *p = values + value_place(row, granule) + byte;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(p));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(p + 8 * DP * 2));
+        return __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    template <int kParts> __device__ __forceinline__ void add(const char *values, uint32_t lane, float *p) {
+        v8 w[kParts][kBlocks * 2];
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+            for (int x = 0; x < kScores; ++x) {
+                const T t = static_cast<T>(p[x]);
+                w[part][x / 8][x % 8] = t;
+                if (part + 1 < kParts) p[x] -= static_cast<float>(t); // exact
+            }
+#pragma unroll
+        for (int d = 0; d < kD; ++d)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const v8 v = value(values, lane, b, u, d);
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) acc[d] = mma32(v, w[part][2 * b + u], acc[d]);
+                }
+    }
+    // The elements of a granule that are not finite, one bit each; they become 0.
+    static __device__ __forceinline__ uint32_t take_nonfinite(uint4 &g) {
+        constexpr uint32_t kHalf = Element<T>::kExponent & 0xffffu;
+        uint32_t bits = 0, w[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((w[i / 2] >> (i % 2 * 16) & kHalf) == kHalf) {
+                bits |= 1u << i;
+                w[i / 2] &= ~(0xffffu << (i % 2 * 16));
+            }
+        g = make_uint4(w[0], w[1], w[2], w[3]);
+        return bits;
+    }
+    // Of a key's bits those of this lane's sums: elements 8 i + 4 h .. + 3 of each
+    // 32 (register 4 i + b of acc[d]: bit 8 i + b of word d).
+    static __device__ __forceinline__ uint32_t odd_word(const uint8_t *of_key, int d, uint32_t h) {
+        return *reinterpret_cast<const uint32_t *>(of_key + 4 * d) >> (4 * h) & 0x0f0f0f0fu;
+    }
+};
+
+// f32 on v_mfma_f32_32x32x2_f32: product e of a score step takes elements 8 s +
+// 4 h + e, and register x of the scores is the value product's step x with no
+// rearrangement at all, slot h being key 8 (x / 4) + 4 h + x % 4.
+template <int DP> struct Tile32<float, DP> {
+    static constexpr int kKeys = 32, kSteps = DP / 8, kD = DP / 32, kScores = 16, kGranules = DP / 4, kGranule = 4;
+    static constexpr int kPerThread = kKeys * kGranules / kThreads;
+    f32x4 q[kSteps];
+    f32x16 acc[kD];
+
+    static __device__ __forceinline__ uint32_t key_place(uint32_t key, uint32_t granule) {
+        return key * (DP * 4) + (granule ^ (key & 15)) * 16;
+    }
+    static __device__ __forceinline__ uint32_t value_place(uint32_t key, uint32_t granule) {
+        return key * (DP * 4) + (granule ^ (key >> 2 & 1) * 8) * 16;
+    }
+    static __device__ __forceinline__ uint32_t key(uint32_t h, int x) { return x / 4 * 8 + 4 * h + x % 4; }
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t h, uint32_t D) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] = f32x4{};
+            if (8 * s + 4 * h < D) q[s] = __builtin_bit_cast(f32x4, ld16(row + (8 * s + 4 * h) * 4));
+        }
+    }
+    __device__ __forceinline__ void scores(const char *keys, uint32_t c, uint32_t h, float *s) const {
+        f32x16 r = {};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const f32x4 k = *reinterpret_cast<const f32x4 *>(keys + key_place(c, 2 * i + h));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[i][e], r, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = r[i];
+    }
+    template <int kParts> __device__ __forceinline__ void add(const char *values, uint32_t lane, const float *p) {
+        const uint32_t c = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int d = 0; d < kD; ++d)
+#pragma unroll
+            for (int x = 0; x < kScores; ++x) {
+                const float v = *reinterpret_cast<const float *>(values + value_place(key(h, x), 8 * d + c / 4) + c % 4 * 4);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[x], acc[d], 0, 0, 0);
+            }
+    }
+    static __device__ __forceinline__ uint32_t take_nonfinite(uint4 &g) {
+        uint32_t bits = 0, w[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if ((w[i] & 0x7f800000u) == 0x7f800000u) {
+                bits |= 1u << i;
+                w[i] = 0;
+            }
+        g = make_uint4(w[0], w[1], w[2], w[3]);
+        return bits;
+    }
+    static __device__ __forceinline__ uint32_t odd_word(const uint8_t *of_key, int d, uint32_t h) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(of_key + 8 * d); // a byte for each granule of 4
+        const uint32_t lo = w.x >> (8 * h), hi = w.y >> (8 * h);
+        return (lo & 15u) | (lo >> 8 & 15u << 8) | (hi & 15u) << 16 | (hi & 15u << 16) << 8;
+    }
+};
+
+constexpr uint32_t kTileRows = 32 * kWaves;
+
+// 128 rows of one sequence and kv head per workgroup, 32 a wavefront, all
+// against the same keys, which pass through two LDS buffers: a tile's rows are
+// loaded into registers during the last one's products and stored after them.
+// grid: row tiles x splits x kv heads, the heads fastest; the tiles with the
+// most keys first.
+template <typename T, int DP, int kParts>
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attention_tiles_kernel(AttentionArgs A) {
+    using Tile = Tile32<T, DP>;
+    constexpr float kLift = Element<T>::kLift;
+    constexpr uint32_t kTileBytes = Tile::kKeys * DP * sizeof(T), kN = Tile::kPerThread;
+    constexpr uint32_t kBits = Tile::kKeys * Tile::kGranules;
+    extern __shared__ __align__(16) char lds[]; // keys, values; keys, values; bits, bits
+    __shared__ uint32_t odd_s[2];               // whether a buffer's bits are set
+    uint8_t *const bits = reinterpret_cast<uint8_t *>(lds) + 4 * kTileBytes;
+    const PagedArgs &a = A.a;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
+    const uint32_t G = A.group.d, D = a.head_dim;
+    bool bad = false;
+    Job job;
+    if (!find_job<kTileRows, Tile::kKeys>(A, gridDim.x - 1 - blockIdx.x, job, bad)) {
+        if (bad && tid == 0) atomicOr(A.status, STATUS_BAD_PAGE);
+        return;
+    }
+    const uint32_t w0 = job.r0 + 32 * wave, w1 = w0 + 32 < job.r1 ? w0 + 32 : job.r1; // this wavefront's rows
+    const bool active = w0 < job.r1;
+    const int32_t lo = job.lo, hi = job.hi;
+    const uint32_t row = w0 + c < job.r1 ? w0 + c : job.r1 - 1, token = A.group.div(row);
+    const uint32_t head = job.kvh * G + row - token * G;
+    const int32_t p = job.before + static_cast<int32_t>(token);
+    const int32_t p_first = job.before + static_cast<int32_t>(A.group.div(active ? w0 : row));
+    const int32_t p_last = job.before + static_cast<int32_t>(A.group.div(active ? w1 - 1 : row));
+    const bool bounded = A.window != kUnbounded;
+    const int32_t window = static_cast<int32_t>(A.window);
+    const int32_t from = bounded ? p - window + 1 : 0;
+    // what every row of the workgroup sees, what every row of the wavefront, and
+    // what any of these
+    const int32_t block_hi = job.before + static_cast<int32_t>(A.group.div(job.r0)) + 1;
+    const int32_t block_lo = bounded ? job.before + static_cast<int32_t>(A.group.div(job.r1 - 1)) - window + 1 : 0;
+    const int32_t all_lo = bounded ? p_last - window + 1 : 0, all_hi = p_first + 1;
+    const int32_t any_lo = bounded ? p_first - window + 1 : 0, any_hi = active ? p_last + 1 : 0;
+
+    Tile tile;
+    tile.load_q(A.q + (job.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), h, D);
+#pragma unroll
+    for (int d = 0; d < Tile::kD; ++d) tile.acc[d] = f32x16{};
+    float top = kNegInf, mass = 0.0f;
+    uint32_t spoiled[Tile::kD] = {}; // sums that met a value that is not finite
+
+    // staging: this thread's granule of kN consecutive keys of a tile
+    const uint32_t granule = tid % Tile::kGranules, key0 = tid / Tile::kGranules * kN;
+    const uint8_t *kp = a.k + job.kvh * a.head_bytes + granule * 16, *vp = a.v + job.kvh * a.head_bytes + granule * 16;
+    const uint32_t *table = a.table + static_cast<uint64_t>(job.index) * a.table_stride;
+    const bool has = D == DP || granule * Tile::kGranule < D;
+    // tiles start at multiples of 4, so where the page size is one too, so do
+    // groups of four keys in their page
+    const bool grouped = a.page.d % 4 == 0;
+    constexpr uint32_t kStep = kN < 4 ? kN : 4;
+    uint32_t page[kN];
+    uint4 kr[kN], vr[kN];
+    auto look_up = [&](int32_t base) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) {
+            const int32_t j = base + static_cast<int32_t>(key0 + i);
+            if (grouped && i % kStep) page[i] = page[i - 1];
+            else page[i] = table[a.page.div(j < hi ? j : hi - 1)];
+        }
+    };
+    auto fetch = [&](int32_t base) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) {
+            const int32_t j = base + static_cast<int32_t>(key0 + i);
+            kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+            if (has && j < hi) {
+                const uint64_t at = position_offset(a, page[i], j - a.page.div(j) * a.page.d, bad);
+                kr[i] = ld16(kp + at);
+                vr[i] = ld16(vp + at);
+            }
+        }
+    };
+    // Infinities and NaN among the values of a tile that some row sees only in
+    // part: a zero weight would not keep them out of that row's sums. They are
+    // stored as 0 with a bit each; the rows that see one get NaN.
+    auto store = [&](int32_t base, uint32_t to) {
+        char *at = lds + to * 2 * kTileBytes;
+        const bool partly = base < block_lo || base + Tile::kKeys > block_hi;
+        uint32_t any = 0;
+        if (partly) {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) {
+                const uint32_t b = Tile::take_nonfinite(vr[i]);
+                bits[to * kBits + (key0 + i) * Tile::kGranules + granule] = b;
+                any |= b;
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) {
+            *reinterpret_cast<uint4 *>(at + Tile::key_place(key0 + i, granule)) = kr[i];
+            *reinterpret_cast<uint4 *>(at + kTileBytes + Tile::value_place(key0 + i, granule)) = vr[i];
+        }
+        if (any) odd_s[to] = 1;
+    };
+    if (tid < 2) odd_s[tid] = 0;
+    __syncthreads();
+    if (lo < hi) {
+        look_up(lo);
+        fetch(lo);
+        look_up(lo + Tile::kKeys);
+        store(lo, 0);
+    }
+    uint32_t buffer = 0;
+    for (int32_t base = lo; base < hi; base += Tile::kKeys, buffer ^= 1) {
+        __syncthreads(); // this buffer is written, the other one read
+        const bool odd = odd_s[buffer];
+        const bool more = base + Tile::kKeys < hi;
+        if (more) {
+            fetch(base + Tile::kKeys);
+            look_up(base + 2 * Tile::kKeys);
+        }
+        const char *keys = lds + buffer * 2 * kTileBytes, *values = keys + kTileBytes;
+        if (base < any_hi && base + Tile::kKeys > any_lo) {
+            float s[Tile::kScores];
+            tile.scores(keys, c, h, s);
+            float high = kNegInf;
+            log2_scores<Tile::kScores>(A, s);
+            if (base < all_lo || base + Tile::kKeys > all_hi) {
+#pragma unroll
+                for (int x = 0; x < Tile::kScores; ++x) {
+                    const int32_t j = base + static_cast<int32_t>(Tile::key(h, x));
+                    s[x] = j <= p && j >= from && j < hi ? s[x] : kNegInf;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < Tile::kScores; ++x) high = fmaxf(high, s[x]);
+            uint32_t u, v;
+            lane_pair_u32<32>(__builtin_bit_cast(uint32_t, high), u, v);
+            high = fmaxf(__builtin_bit_cast(float, u), __builtin_bit_cast(float, v));
+            const float next = fmaxf(top, high), at = next == kNegInf ? 0.0f : next;
+            const float shrink = exp2_fast(top - at);
+            float sum = 0.0f;
+#pragma unroll
+            for (int x = 0; x < Tile::kScores; ++x) {
+                s[x] = exp2_fast(s[x] - at + kLift);
+                sum += s[x];
+            }
+            top = next;
+            mass = mass * shrink + sum; // this lane's keys
+            if (__any(shrink != 1.0f))
+#pragma unroll
+                for (int d = 0; d < Tile::kD; ++d) tile.acc[d] *= shrink;
+            tile.template add<kParts>(values, lane, s);
+            if (odd)
+#pragma unroll 1
+                for (int32_t j = base > from ? base : from; j <= p && j < base + Tile::kKeys && j < hi; ++j)
+#pragma unroll
+                    for (int d = 0; d < Tile::kD; ++d)
+                        spoiled[d] |= Tile::odd_word(bits + buffer * kBits + (j - base) * Tile::kGranules, d, h);
+        }
+        if (more) store(base + Tile::kKeys, buffer ^ 1);
+        if (odd) {
+            __syncthreads();
+            if (tid == 0) odd_s[buffer] = 0;
+        }
+    }
+    if (__any(bad) && lane == 0) atomicOr(A.status, STATUS_BAD_PAGE);
+    uint32_t u, v;
+    lane_pair_u32<32>(__builtin_bit_cast(uint32_t, mass), u, v);
+    mass = __builtin_bit_cast(float, u) + __builtin_bit_cast(float, v);
+    if (!active || w0 + c >= job.r1) return;
+#pragma unroll
+    for (int d = 0; d < Tile::kD; ++d)
+        if (spoiled[d])
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (spoiled[d] >> (i / 4 * 8 + i % 4) & 1) tile.acc[d][i] = __builtin_nanf("");
+#pragma unroll
+    for (int d = 0; d < Tile::kD; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t at = 32 * d + 8 * i + 4 * h;
+            if (at < D)
+                finish(A, job, kTileRows, 32 * wave + c, head, job.start + token, at, top, mass,
+                       f32x4{tile.acc[d][4 * i], tile.acc[d][4 * i + 1], tile.acc[d][4 * i + 2], tile.acc[d][4 * i + 3]},
+                       kLift);
+        }
 }
 
 // A split tile's sums joined: DP / 4 lanes hold a row of one head, kGroups such
@@ -597,7 +956,8 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs 
 
 // A split is worth its second launch and its sums' way through memory where
 // the tiles alone leave CUs idle; never into pieces below one unit of keys.
-constexpr uint32_t kFill = 2048; // workgroups that a split aims at
+constexpr uint32_t kFillRows = 2048, kFillTiles = 512; // workgroups that a split aims at
+constexpr uint32_t kRowsMost = 16; // rows of a sequence that the 16-row kernel takes
 
 // Scratch of a split call: stats, then sums.
 struct Scratch {
@@ -613,14 +973,12 @@ uint64_t tiles_of(const PagedArgs &a, uint32_t group, uint32_t tile_rows) {
     return static_cast<uint64_t>(a.tokens) * group / tile_rows + (a.sequences < a.tokens ? a.sequences : a.tokens);
 }
 
-uint32_t splits_of(const PagedArgs &a, uint64_t tiles, uint32_t unit) {
+uint32_t splits_of(const PagedArgs &a, uint64_t tiles, uint32_t unit, uint32_t fill) {
     const uint64_t blocks = tiles * a.kv_heads;
     const uint32_t most = div_up(a.max_length, unit);
-    const uint64_t want = (kFill + blocks - 1) / blocks;
+    const uint64_t want = (fill + blocks - 1) / blocks;
     return static_cast<uint32_t>(want < most ? want : most);
 }
-
-constexpr uint32_t rows_unit(uint32_t type) { return (type == FMX_TYPE_F32 ? 16 : 32) * kWaves; }
 
 template <typename T, int DP> int launch_join(const AttentionArgs &A, uint64_t tiles, uint32_t tile_rows, uint32_t unit,
                                               hipStream_t s) {
@@ -636,26 +994,43 @@ template <typename T, int DP> int launch_join(const AttentionArgs &A, uint64_t t
     return FMX_OK;
 }
 
-template <typename T, int DP, int kParts> int launch_rows(AttentionArgs A, uint8_t *scratch, uint32_t type, hipStream_t s) {
-    const uint64_t tiles = tiles_of(A.a, A.group.d, kRows);
-    const uint32_t unit = rows_unit(type);
-    A.splits = splits_of(A.a, tiles, unit);
+// Which kernel takes a call, and what it splits into: 16 rows a workgroup while
+// a sequence's rows fit few such tiles, else 128.
+struct Plan {
+    uint32_t tile_rows, unit, splits;
+    uint64_t tiles;
+};
+Plan plan_of(const PagedArgs &a, uint32_t type, uint32_t group) {
+    Plan p;
+    const bool rows = static_cast<uint64_t>(a.max_new) * group <= kRowsMost;
+    p.tile_rows = rows ? kRows : kTileRows;
+    p.unit = rows ? (type == FMX_TYPE_F32 ? 16 : 32) * kWaves
+                  : type == FMX_TYPE_F32 || a.head_dim > 128 ? 32 : 64;
+    p.tiles = tiles_of(a, group, p.tile_rows);
+    p.splits = splits_of(a, p.tiles, p.unit, rows ? kFillRows : kFillTiles);
+    return p;
+}
+
+template <typename T, int DP, int kParts> int launch_one(AttentionArgs A, uint8_t *scratch, uint32_t type, hipStream_t s) {
+    const Plan p = plan_of(A.a, type, A.group.d);
+    A.splits = p.splits;
     A.stats = reinterpret_cast<float2 *>(scratch);
-    A.parts = reinterpret_cast<float *>(scratch + scratch_of(tiles, A.a.kv_heads, A.splits, kRows, A.a.head_dim).stats);
-    const uint64_t blocks = tiles * A.a.kv_heads * A.splits;
+    A.parts = reinterpret_cast<float *>(scratch + scratch_of(p.tiles, A.a.kv_heads, p.splits, p.tile_rows, A.a.head_dim).stats);
+    const uint64_t blocks = p.tiles * A.a.kv_heads * p.splits;
     if (blocks > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
-    const size_t lds = kWaves * kRows * (DP + 4) * sizeof(float);
-    const auto kernel = attention_rows_kernel<T, DP, kParts>;
+    const bool rows = p.tile_rows == kRows;
+    const size_t lds = rows ? kWaves * kRows * (DP + 4) * sizeof(float) : Tile32<T, DP>::kKeys * (4 * DP * sizeof(T) + 2 * Tile32<T, DP>::kGranules);
+    const auto kernel = rows ? attention_rows_kernel<T, DP, kParts> : attention_tiles_kernel<T, DP, kParts>;
     if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), lds, s, A);
     FMX_LAUNCH_CHECK();
-    return launch_join<T, DP>(A, tiles, kRows, unit, s);
+    return launch_join<T, DP>(A, p.tiles, p.tile_rows, p.unit, s);
 }
 
 template <typename T, int kParts> int launch_dim(const AttentionArgs &A, uint8_t *scratch, uint32_t type, hipStream_t s) {
-    if (A.a.head_dim <= 64) return launch_rows<T, 64, kParts>(A, scratch, type, s);
-    if (A.a.head_dim <= 128) return launch_rows<T, 128, kParts>(A, scratch, type, s);
-    return launch_rows<T, 256, kParts>(A, scratch, type, s);
+    if (A.a.head_dim <= 64) return launch_one<T, 64, kParts>(A, scratch, type, s);
+    if (A.a.head_dim <= 128) return launch_one<T, 128, kParts>(A, scratch, type, s);
+    return launch_one<T, 256, kParts>(A, scratch, type, s);
 }
 
 template <typename T> int launch_type(const AttentionArgs &A, uint8_t *scratch, uint32_t type, hipStream_t s) {
@@ -666,9 +1041,8 @@ template <typename T> int launch_type(const AttentionArgs &A, uint8_t *scratch, 
 } // namespace
 
 uint64_t attention_paged_scratch(const PagedArgs &a, uint32_t type, uint32_t heads) {
-    const uint64_t tiles = tiles_of(a, heads / a.kv_heads, kRows);
-    const uint32_t splits = splits_of(a, tiles, rows_unit(type));
-    return splits > 1 ? scratch_of(tiles, a.kv_heads, splits, kRows, a.head_dim).total : 0;
+    const Plan p = plan_of(a, type, heads / a.kv_heads);
+    return p.splits > 1 ? scratch_of(p.tiles, a.kv_heads, p.splits, p.tile_rows, a.head_dim).total : 0;
 }
 
 int attention_paged(const PagedArgs &a, uint32_t type, const AttentionCall &c, hipStream_t s) {
