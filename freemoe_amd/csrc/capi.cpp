@@ -736,7 +736,7 @@ int fmx_attention_paged(const fmx_paged_cache *cache, const fmx_paged_batch *bat
     if (int rc = fault_gate()) return rc;
     PagedArgs a;
     if (int rc = prepare_paged(cache, batch, &a)) return rc;
-    if (!options || !std::isfinite(options->scale) || !(options->softcap >= 0.0) || !std::isfinite(options->softcap))
+    if (!options || !(std::fabs(options->scale) < 0x1p100) || !(options->softcap >= 0.0) || !(options->softcap < 0x1p100))
         return FMX_ERR_INVALID_ARGUMENT;
     if (out_type != FMX_TYPE_F32 && out_type != cache->type) return FMX_ERR_UNSUPPORTED_QUANTISATION;
     if (heads == 0 || heads > 65535 || heads % cache->kv_heads) return FMX_ERR_SHAPE_MISMATCH;

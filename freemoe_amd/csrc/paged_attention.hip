@@ -33,8 +33,9 @@ struct AttentionArgs {
     uint64_t q_bytes, out_bytes; // row strides
     uint32_t heads;
     FastDiv group;               // query heads of a kv head
-    float scale;                 // times log2 e (softcap: 1 / softcap times the plain one)
-    float softcap;               // times log2 e, or 0
+    float scale, softcap;        // scale / softcap and softcap, or 0
+    float per_score;             // log 2 units of a score, never negative: q's sign is turned instead
+    bool negate;
     uint32_t window;             // or kUnbounded
     const float *sinks;
     uint32_t out_type;
@@ -105,20 +106,26 @@ __device__ __forceinline__ bool find_job(const AttentionArgs &A, uint32_t block,
     return true;
 }
 
-// Element types: how many 16-bit parts carry a weight to f32 accuracy, and the
+// Element types: how many 16-bit parts carry a weight to f32 accuracy; kSlack,
+// by how many powers of two a score may pass the maximum its row's sums are
+// kept at before they are brought to a new one (any number near the maximum
+// serves, and most tiles bring a slightly larger one for some row); kLift, the
 // power of two the weights are kept at. A half's range ends at 2^-24, which
-// would cost small weights their low bits: its weights are kept 2^15 times as
-// large (at most 32768; the sum carries the same factor).
+// would cost small weights their low bits: its weights are kept 2^9 times as
+// large, 2^15 at most with the slack (the sum carries the same factor).
 template <typename T> struct Element;
-template <> struct Element<float> { static constexpr int kParts = 1; static constexpr float kLift = 0.0f; };
+template <> struct Element<float> {
+    static constexpr int kParts = 1;
+    static constexpr float kLift = 0.0f, kSlack = 8.0f;
+};
 template <> struct Element<_Float16> {
     static constexpr int kParts = 2;
-    static constexpr float kLift = 15.0f;
+    static constexpr float kLift = 9.0f, kSlack = 6.0f;
     static constexpr uint32_t kExponent = 0x7c007c00u;
 };
 template <> struct Element<__bf16> {
     static constexpr int kParts = 3;
-    static constexpr float kLift = 0.0f;
+    static constexpr float kLift = 0.0f, kSlack = 8.0f;
     static constexpr uint32_t kExponent = 0x7f807f80u;
 };
 
@@ -169,11 +176,12 @@ template <typename T, int DP> struct Tile16 {
 
     static __device__ __forceinline__ uint32_t key(uint32_t g, int x) { return (x < 4 ? 0 : 12) + 4 * g + x; }
 
-    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t g, uint32_t D) {
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t g, uint32_t D, bool negate) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             q[s] = v8{};
             if (32 * s + 8 * g < D) q[s] = __builtin_bit_cast(v8, ld16(row + (32 * s + 8 * g) * 2));
+            if (negate) q[s] = -q[s];
         }
     }
     __device__ __forceinline__ void load(const uint8_t *kp, const uint8_t *vp, const uint64_t *offset, uint32_t c,
@@ -295,11 +303,12 @@ template <int DP> struct Tile16<float, DP> {
 
     static __device__ __forceinline__ uint32_t key(uint32_t g, int x) { return 4 * g + x; }
 
-    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t g, uint32_t D) {
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t g, uint32_t D, bool negate) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             q[s] = f32x4{};
             if (16 * s + 4 * g < D) q[s] = __builtin_bit_cast(f32x4, ld16(row + (16 * s + 4 * g) * 4));
+            if (negate) q[s] = -q[s];
         }
     }
     __device__ __forceinline__ void load(const uint8_t *kp, const uint8_t *vp, const uint64_t *offset, uint32_t c,
@@ -365,13 +374,12 @@ template <int DP> struct Tile16<float, DP> {
     }
 };
 
-// Scores in units of log 2 from q . k.
-template <int kN> __device__ __forceinline__ void log2_scores(const AttentionArgs &A, float *s) {
-#pragma unroll
-    for (int x = 0; x < kN; ++x) s[x] *= A.scale;
+// Scores from q . k, in units of 1 / per_score of log 2: q . k itself, or the
+// capped score.
+template <int kN> __device__ __forceinline__ void cap_scores(const AttentionArgs &A, float *s) {
     if (A.softcap != 0.0f)
 #pragma unroll
-        for (int x = 0; x < kN; ++x) s[x] = tanhf(s[x]) * A.softcap;
+        for (int x = 0; x < kN; ++x) s[x] = tanhf(s[x] * A.scale) * A.softcap;
 }
 
 __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, uint32_t type, f32x4 x) {
@@ -447,7 +455,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
     const int32_t all_lo = bounded ? p_last - window + 1 : 0, all_hi = p_first + 1;
 
     Tile tile;
-    tile.load_q(A.q + (job.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), g, D);
+    tile.load_q(A.q + (job.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), g, D, A.negate);
 #pragma unroll
     for (int m = 0; m < Tile::kE; ++m) tile.acc[m] = f32x4{};
     float top = kNegInf, mass = 0.0f;
@@ -466,7 +474,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
         float s[Tile::kScores];
         tile.scores(s);
         if (base + Tile::kKeys > hi) tile.clear_values(g, hi - base);
-        log2_scores<Tile::kScores>(A, s);
+        cap_scores<Tile::kScores>(A, s);
         float high = kNegInf;
         if (base < all_lo || base + Tile::kKeys > all_hi) {
             bool seen[Tile::kScores];
@@ -480,13 +488,13 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
         }
 #pragma unroll
         for (int x = 0; x < Tile::kScores; ++x) high = fmaxf(high, s[x]);
-        high = row_max(high);
+        high = row_max(high) * A.per_score;
         const float next = fmaxf(top, high), at = next == kNegInf ? 0.0f : next;
-        const float shrink = exp2_fast(top - at);
+        const float shrink = exp2_fast(top - at), shift = kLift - at;
         float w[Tile::kScores], sum = 0.0f;
 #pragma unroll
         for (int x = 0; x < Tile::kScores; ++x) {
-            w[x] = exp2_fast(s[x] - at + kLift);
+            w[x] = exp2_fast(fma_rn(s[x], A.per_score, shift));
             sum += w[x];
         }
         top = next;
@@ -569,11 +577,12 @@ template <typename T, int DP> struct Tile32 {
     static __device__ __forceinline__ uint32_t key(uint32_t h, int x) {
         return x / 16 * 32 + x % 16 / 4 * 8 + 4 * h + x % 4;
     }
-    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t h, uint32_t D) {
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t h, uint32_t D, bool negate) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             q[s] = v8{};
             if (16 * s + 8 * h < D) q[s] = __builtin_bit_cast(v8, ld16(row + (16 * s + 8 * h) * 2));
+            if (negate) q[s] = -q[s];
         }
     }
     __device__ __forceinline__ void scores(const char *keys, uint32_t c, uint32_t h, float *s) const {
@@ -655,11 +664,12 @@ template <int DP> struct Tile32<float, DP> {
         return key * (DP * 4) + (granule ^ (key >> 2 & 1) * 8) * 16;
     }
     static __device__ __forceinline__ uint32_t key(uint32_t h, int x) { return x / 4 * 8 + 4 * h + x % 4; }
-    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t h, uint32_t D) {
+    __device__ __forceinline__ void load_q(const uint8_t *row, uint32_t h, uint32_t D, bool negate) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             q[s] = f32x4{};
             if (8 * s + 4 * h < D) q[s] = __builtin_bit_cast(f32x4, ld16(row + (8 * s + 4 * h) * 4));
+            if (negate) q[s] = -q[s];
         }
     }
     __device__ __forceinline__ void scores(const char *keys, uint32_t c, uint32_t h, float *s) const {
@@ -745,7 +755,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attention_tiles_k
     const int32_t any_lo = bounded ? p_first - window + 1 : 0, any_hi = active ? p_last + 1 : 0;
 
     Tile tile;
-    tile.load_q(A.q + (job.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), h, D);
+    tile.load_q(A.q + (job.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), h, D, A.negate);
 #pragma unroll
     for (int d = 0; d < Tile::kD; ++d) tile.acc[d] = f32x16{};
     float top = kNegInf, mass = 0.0f;
@@ -766,19 +776,31 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attention_tiles_k
 #pragma unroll
         for (uint32_t i = 0; i < kN; ++i) {
             const int32_t j = base + static_cast<int32_t>(key0 + i);
-            if (grouped && i % kStep) page[i] = page[i - 1];
-            else page[i] = table[a.page.div(j < hi ? j : hi - 1)];
+            if (i % kStep == 0 || !grouped) page[i] = table[a.page.div(j < hi ? j : hi - 1)];
         }
     };
     auto fetch = [&](int32_t base) {
+        uint64_t at[kN];
 #pragma unroll
         for (uint32_t i = 0; i < kN; ++i) {
             const int32_t j = base + static_cast<int32_t>(key0 + i);
-            kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-            if (has && j < hi) {
-                const uint64_t at = position_offset(a, page[i], j - a.page.div(j) * a.page.d, bad);
-                kr[i] = ld16(kp + at);
-                vr[i] = ld16(vp + at);
+            if (i % kStep == 0 || !grouped) at[i] = position_offset(a, page[i], j - a.page.div(j) * a.page.d, bad);
+            else at[i] = at[i - 1] + a.position_bytes;
+        }
+        if (has && base + Tile::kKeys <= hi) {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) {
+                kr[i] = ld16(kp + at[i]);
+                vr[i] = ld16(vp + at[i]);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) {
+                kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+                if (has && base + static_cast<int32_t>(key0 + i) < hi) {
+                    kr[i] = ld16(kp + at[i]);
+                    vr[i] = ld16(vp + at[i]);
+                }
             }
         }
     };
@@ -826,7 +848,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attention_tiles_k
             float s[Tile::kScores];
             tile.scores(keys, c, h, s);
             float high = kNegInf;
-            log2_scores<Tile::kScores>(A, s);
+            cap_scores<Tile::kScores>(A, s);
             if (base < all_lo || base + Tile::kKeys > all_hi) {
 #pragma unroll
                 for (int x = 0; x < Tile::kScores; ++x) {
@@ -838,20 +860,23 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attention_tiles_k
             for (int x = 0; x < Tile::kScores; ++x) high = fmaxf(high, s[x]);
             uint32_t u, v;
             lane_pair_u32<32>(__builtin_bit_cast(uint32_t, high), u, v);
-            high = fmaxf(__builtin_bit_cast(float, u), __builtin_bit_cast(float, v));
-            const float next = fmaxf(top, high), at = next == kNegInf ? 0.0f : next;
-            const float shrink = exp2_fast(top - at);
+            high = fmaxf(__builtin_bit_cast(float, u), __builtin_bit_cast(float, v)) * A.per_score;
+            const bool raise = high > top + Element<T>::kSlack; // (also from -inf)
+            if (__any(raise)) {
+                const float next = raise ? high : top, shrink = raise ? exp2_fast(top - high) : 1.0f;
+                top = next;
+                mass *= shrink;
+#pragma unroll
+                for (int d = 0; d < Tile::kD; ++d) tile.acc[d] *= shrink;
+            }
+            const float shift = kLift - (top == kNegInf ? 0.0f : top);
             float sum = 0.0f;
 #pragma unroll
             for (int x = 0; x < Tile::kScores; ++x) {
-                s[x] = exp2_fast(s[x] - at + kLift);
+                s[x] = exp2_fast(fma_rn(s[x], A.per_score, shift));
                 sum += s[x];
             }
-            top = next;
-            mass = mass * shrink + sum; // this lane's keys
-            if (__any(shrink != 1.0f))
-#pragma unroll
-                for (int d = 0; d < Tile::kD; ++d) tile.acc[d] *= shrink;
+            mass += sum; // this lane's keys
             tile.template add<kParts>(values, lane, s);
             if (odd)
 #pragma unroll 1
@@ -1056,8 +1081,15 @@ int attention_paged(const PagedArgs &a, uint32_t type, const AttentionCall &c, h
     A.group = FastDiv(c.heads / a.kv_heads);
     constexpr double kLog2e = 1.4426950408889634;
     const double cap = c.options.softcap;
-    A.scale = static_cast<float>(cap != 0.0 ? c.options.scale / cap : c.options.scale * kLog2e);
-    A.softcap = static_cast<float>(cap * kLog2e);
+    A.negate = c.options.scale < 0.0;
+    const double scale = A.negate ? -c.options.scale : c.options.scale;
+    A.scale = static_cast<float>(cap != 0.0 ? scale / cap : 0.0);
+    A.softcap = static_cast<float>(cap);
+    A.per_score = static_cast<float>(cap != 0.0 ? kLog2e : scale * kLog2e);
+    if (A.per_score == 0.0f) { // a scale of 0: all scores alike (0 times a hidden one's -inf would be NaN)
+        A.softcap = 1.0f;
+        A.per_score = static_cast<float>(kLog2e);
+    }
     A.window = c.options.window == 0 || c.options.window > 0x7fffffffu ? kUnbounded : c.options.window;
     A.sinks = c.options.sinks;
     A.out_type = c.out_type;

@@ -176,6 +176,10 @@ ATTENTION = {
     "peaked": (4, 2, 128, BF16, F32, 16, [5, 70], [300, 70], dict(peak=6.0)),
     "peaked_f16": (4, 2, 128, F16, F32, 16, [5, 70], [300, 70], dict(peak=6.0)),
     "more_tokens_than_positions": (2, 1, 64, BF16, F32, 16, [5, 3], [2, 0], {}),
+    "negative_scale": (4, 2, 64, BF16, F32, 16, [1, 70], [90, 70], dict(scale=-0.2)),
+    "no_scale": (4, 2, 64, F16, F32, 16, [1, 70], [90, 70], dict(scale=0.0)),
+    "rising_scores": (2, 1, 64, F16, F32, 16, [3, 40], [700, 400], dict(rise=True)),
+    "rising_scores_bf16": (2, 1, 128, BF16, BF16, 16, [3, 40], [700, 400], dict(rise=True)),
     "many_sequences": (2, 1, 32, F32, F32, 8, [1 + i % 2 for i in range(140)], [2 + i % 50 for i in range(140)], {}),
 }
 
@@ -187,6 +191,12 @@ def attention_case(name):
     P = ref.Paged(counts, [max(n, 0) for n in lengths], G, D, ps, tc, 17, by_head=len(counts) % 2 == 0,
                   pad=8 if D % 16 else 0)
     q = (torch.randn(P.tokens, H, D, generator=P.g) * peak).to(tc)
+    if options.pop("rise", False):  # scores that grow along the sequence, so that every tile brings a new maximum
+        for i, n in enumerate(P.lengths):
+            j = torch.arange(n)
+            at = P.table[i].long()[j // ps], j % ps
+            P.pools[0][1][at] = (P.pools[0][1][at].float() * 0.1 + j[:, None, None] * 0.05).to(tc)
+        q = (0.5 + torch.rand(q.shape, generator=P.g)).to(tc)
     if options.get("sinks"):
         options["sinks"] = torch.randn(H, generator=P.g) * 2
     return P, q, tout, options
@@ -219,7 +229,8 @@ def test_attention_paged(gpu, name):
     assert sv.status(ws) == 0
     got = out.cpu()
     assert (got[P.starts[-1]:] == 7.0).all() and (got[:, H * D:] == 7.0).all()
-    check_attention(P, q, got[:, :H * D].unflatten(1, (H, D)), options, tout, 1.0 / math.sqrt(D))
+    scale = options.pop("scale", 1.0 / math.sqrt(D))
+    check_attention(P, q, got[:, :H * D].unflatten(1, (H, D)), options, tout, scale)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
