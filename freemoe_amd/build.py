@@ -20,7 +20,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libfmx.so"
 
 SOURCES = ["capi.cpp", "quant.hip", "matvec.hip", "gemm.hip", "moe.hip", "down_pair_q4k.hip", "bucket.hip",
-           "prefill.hip", "attention.hip", "rope.hip", "paged_attention.hip", "sample.hip"]
+           "prefill.hip", "attention.hip", "rope.hip", "paged_attention.hip",
+           "attention_f32.hip", "attention_f16.hip", "attention_bf16.hip", "sample.hip"]
 
 HIP_FLAGS = [
     "--offload-arch=gfx950",
