@@ -7,12 +7,13 @@
 // order, so what is kept is the shortest of three prefixes and its mass the
 // least of three masses, and the token is the first whose cumulated mass
 // exceeds uniform x that mass. Nothing is sorted: a place in the order where a
-// count or a mass crosses a target is found by a histogram of masses over
-// equal steps of x, then among the elements of the one step that holds it.
+// count or a mass crosses a target is found by a histogram over equal steps of
+// x, then among the elements of the one step that holds it, every one against
+// every other. A small top-k needs no masses but its own: the steps down to
+// the k-th logit are taken out at once.
 //
 // Masses are integers in steps of 2^-44: their sums do not depend on the order
-// of the additions (LDS atomics, whichever wavefront comes first), and what
-// they lose is 2^-45 of the largest weight per token.
+// of the additions (LDS atomics, whichever wavefront comes first).
 #include "paged.hpp"
 
 namespace fmx {
@@ -21,11 +22,14 @@ namespace {
 
 constexpr uint32_t kThreads = 1024;
 constexpr uint32_t kWaves = kThreads / 64;
-constexpr uint32_t kBins = 2048;     // of the first histogram
-constexpr uint32_t kFineBins = 1024; // of those inside one of its steps
-constexpr uint32_t kList = 1024;     // elements compared pair by pair
+constexpr uint32_t kBins = 2048;
+constexpr uint32_t kList = 1024;  // elements compared pair by pair
 constexpr uint32_t kMassBits = 44;
 static_assert(kSampleMaxVocab <= 1u << 18, "sums of that many masses of at most 2^44 stay below 2^63");
+
+// A top-k up to here is taken out by counts (the list holds it and the rest of
+// its last step).
+constexpr uint32_t kCountedTopK = 512;
 
 struct SampleArgs {
     const float *logits;
@@ -53,11 +57,40 @@ __device__ __forceinline__ double exp2_table(double t, const double *table) {
     return ldexp(fma(s * r, base, base), i >> 6);
 }
 
-// An element's place in the order.
-struct Place {
-    float x;
-    uint32_t id;
+// A row's weights. Those of at least 2^-8 of the largest, and all that min-p
+// might keep, come from double arithmetic; the others, a body that matters by
+// its sum, from v_exp_f32 on a product carried to 2^-24 of the exponent (about
+// 2^-20 of each weight, at most 2^-28 of the largest, in either direction).
+// Weights below 2^-46 are none.
+struct Weights {
+    float M, c_hi, c_lo, heavy; // log 2 units per logit in two floats; exponents from `heavy` on in double
+    double M_d, c;
+    const double *table;
+
+    __device__ __forceinline__ float exponent(float x) const {
+        const float d = x - M;
+        return fma_rn(d, c_hi, d * c_lo);
+    }
+    // d = -inf times a zero c is NaN: no weight, as any exponent not above -46
+    static __device__ __forceinline__ bool any(float t) { return t > -46.0f; }
+    __device__ __forceinline__ uint64_t light(float t) const {
+        return static_cast<uint64_t>(static_cast<uint32_t>(fma_rn(__builtin_amdgcn_exp2f(t), 0x1p40f, 0.5f))) << 4;
+    }
+    __device__ __forceinline__ double exact(float x) const {
+        const double t = (static_cast<double>(x) - M_d) * c;
+        return t > -46.0 ? exp2_table(t, table) : 0.0;
+    }
+    // an integer below 2^45 through the mantissa of 2^52 + it
+    static __device__ __forceinline__ uint64_t mass(double w) {
+        return __builtin_bit_cast(uint64_t, w * 0x1p44 + 0x1p52) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ uint64_t of(float x) const {
+        const float t = exponent(x);
+        if (!any(t)) return 0;
+        return t >= heavy ? mass(exact(x)) : light(t);
+    }
 };
+
 __device__ __forceinline__ bool precedes(float xa, uint32_t ia, float xb, uint32_t ib) {
     return xa > xb || (xa == xb && ia < ib);
 }
@@ -75,8 +108,8 @@ struct Target {
 };
 
 struct Shared {
-    uint64_t mass[kBins], fine_mass[kFineBins], list_mass[kList];
-    uint32_t count[kBins], fine_count[kFineBins];
+    uint64_t mass[kBins], list_mass[kList];
+    uint32_t count[kBins];
     float list_x[kList];
     uint32_t list_id[kList];
     double table[64];
@@ -85,52 +118,77 @@ struct Shared {
     float wave_a[kWaves], wave_b[kWaves];
     uint32_t wave_id[kWaves];
     bool wave_bad[kWaves];
-    uint32_t n, step, found;
-    Place cut;
-    uint64_t cut_mass;
+    uint32_t n, step;
+    float cut_x;
+    uint32_t cut_id;
+    uint64_t cut_mass, kept_by_min;
 };
 
-// Inclusive sums of n entries, a power of two from kThreads on, in place.
-__device__ void scan_bins(Shared &s, uint64_t *mass, uint32_t *count, uint32_t n) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = n / kThreads;
-    uint64_t m = 0;
-    uint32_t c = 0;
-    for (uint32_t i = 0; i < per; ++i) {
-        m += mass[tid * per + i];
-        c += count[tid * per + i];
+// Steps of x: element x lies in step floor((top - x) * scale), the last one
+// taking the rest; monotonic in x, so the steps are stretches of the order.
+// (An infinite difference at an infinite temperature: scale 0, step 0.)
+struct Steps {
+    float top, scale;
+    __device__ __forceinline__ uint32_t of(float x) const {
+        const float d = (top - x) * scale;
+        return d < static_cast<float>(kBins - 1) ? static_cast<uint32_t>(d) : d > 0.0f ? kBins - 1 : 0;
     }
-    uint64_t mi = m;
-    uint32_t ci = c;
+};
+
+// Inclusive sums of the steps' masses and counts, in place.
+__device__ __forceinline__ void scan_steps(Shared &s) {
+    constexpr uint32_t kPer = kBins / kThreads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint64_t m[kPer], mi = 0;
+    uint32_t c[kPer], ci = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+        mi += s.mass[tid * kPer + i];
+        ci += s.count[tid * kPer + i];
+        m[i] = mi;
+        c[i] = ci;
+    }
+    const uint64_t own_m = mi;
+    const uint32_t own_c = ci;
+#pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) {
         const uint64_t mo = __shfl_up(mi, d);
         const uint32_t co = __shfl_up(ci, d);
-        if (lane >= d) {
-            mi += mo;
-            ci += co;
-        }
+        mi += lane >= d ? mo : 0;
+        ci += lane >= d ? co : 0;
     }
     if (lane == 63) {
         s.wave_mass[wave] = mi;
         s.wave_count[wave] = ci;
     }
     __syncthreads();
-    mi -= m;
-    ci -= c;
-    for (uint32_t i = 0; i < wave; ++i) {
-        mi += s.wave_mass[i];
-        ci += s.wave_count[i];
+    mi -= own_m;
+    ci -= own_c;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaves; ++i) {
+        mi += i < wave ? s.wave_mass[i] : 0;
+        ci += i < wave ? s.wave_count[i] : 0;
     }
-    for (uint32_t i = 0; i < per; ++i) {
-        mi += mass[tid * per + i];
-        ci += count[tid * per + i];
-        mass[tid * per + i] = mi;
-        count[tid * per + i] = ci;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+        s.mass[tid * kPer + i] = mi + m[i];
+        s.count[tid * kPer + i] = ci + c[i];
     }
     __syncthreads();
 }
 
-// The row, in registers where kHeld elements a thread hold it, else read again
-// at each pass (from L2).
+// The row in memory, one element at a time, for the passes few rows need.
+struct SlowRow {
+    const float *from;
+    uint32_t vocab;
+    template <class F> __device__ __forceinline__ void each(const F &f) const {
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) f(from[i], i);
+    }
+};
+
+// The row: kHeld elements a thread in registers, or (0) read again at each
+// pass, from L2.
 template <uint32_t kHeld> struct Row {
     float held[kHeld ? kHeld : 1];
     const float *from;
@@ -163,41 +221,180 @@ template <uint32_t kHeld> struct Row {
     }
 };
 
-// Steps of x: element x lies in step floor((top - x) * scale), the last one
-// taking the rest; monotonic in x, so the steps are stretches of the order.
-struct Steps {
-    double top, scale;
-    uint32_t last;
-    __device__ __forceinline__ uint32_t of(float x) const {
-        const double d = (top - static_cast<double>(x)) * scale;
-        return d < static_cast<double>(last) ? static_cast<uint32_t>(d) : last;
+__device__ __forceinline__ void put(Shared &s, float x, uint32_t i) {
+    const uint32_t at = atomicAdd(&s.n, 1u);
+    if (at < kList) {
+        s.list_x[at] = x;
+        s.list_id[at] = i;
     }
-};
+}
+
+// Of the listed elements, whose predecessors hold m0 and number c0: the one at
+// which `t` is first met, to s.cut_*.
+__device__ __forceinline__ void rank_list(Shared &s, const Target &t, uint32_t listed, uint64_t m0, uint32_t c0) {
+    const uint32_t tid = threadIdx.x;
+    if (tid < listed) {
+        const float x = s.list_x[tid];
+        const uint32_t id = s.list_id[tid];
+        uint64_t m = m0;
+        uint32_t c = c0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < listed; ++j)
+            if (precedes(s.list_x[j], s.list_id[j], x, id)) {
+                m += s.list_mass[j];
+                ++c;
+            }
+        const uint64_t with = m + s.list_mass[tid];
+        if (t.met(c + 1, with) && !t.met(c, m)) {
+            s.cut_x = x;
+            s.cut_id = id;
+            s.cut_mass = with;
+        }
+    }
+    __syncthreads();
+}
+
+// A stretch of the order with more elements than the list takes, those with lo
+// <= x <= hi: narrowed by finer and finer steps, or, where all are equal,
+// counted off by id. Fills s.cut_* and returns true, or leaves the stretch's
+// bounds, mass and count for the list.
+__device__ __forceinline__ bool narrow(Shared &s, SlowRow row, Weights w, Target t, float &hi, float &lo, uint64_t &m0,
+                                    uint32_t &c0, uint32_t &n) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr float kInf = __builtin_inff();
+    // (the steps' sums have served; their arrays hold the finer ones)
+    const auto bounds = [&](float &a, float &b, auto in) {
+        a = -kInf;
+        b = kInf;
+        row.each([&](float x, uint32_t) {
+            if (in(x) && Weights::any(w.exponent(x))) {
+                a = fmaxf(a, x);
+                b = fminf(b, x);
+            }
+        });
+        for (uint32_t d = 32; d >= 1; d >>= 1) {
+            a = fmaxf(a, __shfl_xor(a, d));
+            b = fminf(b, __shfl_xor(b, d));
+        }
+        __syncthreads();
+        if (lane == 0) {
+            s.wave_a[wave] = a;
+            s.wave_b[wave] = b;
+        }
+        __syncthreads();
+        for (uint32_t i = 0; i < kWaves; ++i) {
+            a = fmaxf(a, s.wave_a[i]);
+            b = fminf(b, s.wave_b[i]);
+        }
+    };
+    while (n > kList) {
+        float a, b;
+        bounds(a, b, [&](float x) { return x <= hi && x >= lo; });
+        if (a == b) {
+            const uint64_t m = w.of(a);
+            uint32_t least = 1, most = n; // the smallest count that meets the target
+            while (least < most) {
+                const uint32_t mid = (least + most) / 2;
+                if (t.met(c0 + mid, m0 + mid * m)) most = mid;
+                else least = mid + 1;
+            }
+            uint32_t left = least;
+            for (uint32_t i0 = 0; i0 < row.vocab; i0 += kThreads) {
+                const uint32_t i = i0 + tid;
+                const bool here = i < row.vocab && row.from[i] == a;
+                const uint64_t vote = __ballot(here);
+                __syncthreads();
+                if (lane == 0) s.wave_count[wave] = __builtin_popcountll(vote);
+                __syncthreads();
+                uint32_t before = 0, all = 0;
+                for (uint32_t k = 0; k < kWaves; ++k) {
+                    before += k < wave ? s.wave_count[k] : 0;
+                    all += s.wave_count[k];
+                }
+                if (left > all) {
+                    left -= all;
+                    continue;
+                }
+                before += __builtin_popcountll(vote & ((uint64_t{1} << lane) - 1));
+                if (here && before + 1 == left) {
+                    s.cut_x = a;
+                    s.cut_id = i;
+                    s.cut_mass = m0 + least * m;
+                }
+                break;
+            }
+            __syncthreads();
+            return true;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < kBins; i += kThreads) {
+            s.mass[i] = 0;
+            s.count[i] = 0;
+        }
+        __syncthreads();
+        const double per = (kBins - 1) / (static_cast<double>(a) - static_cast<double>(b));
+        const auto step_of = [&](float x) {
+            const double d = (static_cast<double>(a) - static_cast<double>(x)) * per;
+            return d < kBins - 1 ? static_cast<uint32_t>(d) : kBins - 1;
+        };
+        row.each([&](float x, uint32_t) {
+            if (!(x <= hi && x >= lo)) return;
+            if (!Weights::any(w.exponent(x))) return;
+            const uint32_t f = step_of(x);
+            atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[f]), w.of(x));
+            atomicAdd(&s.count[f], 1u);
+        });
+        __syncthreads();
+        scan_steps(s);
+        for (uint32_t i = tid; i < kBins; i += kThreads)
+            if (t.met(c0 + s.count[i], m0 + s.mass[i]) && (i == 0 || !t.met(c0 + s.count[i - 1], m0 + s.mass[i - 1])))
+                s.step = i;
+        __syncthreads();
+        const uint32_t f = s.step;
+        const uint64_t fm = f ? s.mass[f - 1] : 0;
+        const uint32_t fc = f ? s.count[f - 1] : 0;
+        n = s.count[f] - fc;
+        m0 += fm;
+        c0 += fc;
+        const float was_hi = hi, was_lo = lo;
+        bounds(hi, lo, [&](float x) { return x <= was_hi && x >= was_lo && step_of(x) == f; });
+    }
+    return false;
+}
 
 // grid: rows.
 template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs A) {
     __shared__ Shared s;
+    constexpr float kInf = __builtin_inff();
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x, V = A.vocab;
     Row<kHeld> row;
     row.from = A.logits + r * A.row_stride;
     row.vocab = V;
     row.load();
+    const SlowRow slow{row.from, V};
     const float temperature = A.p.temperature ? A.p.temperature[r] : 1.0f;
     const uint32_t top_k = A.p.top_k ? A.p.top_k[r] : 0;
     const float top_p = A.p.top_p ? A.p.top_p[r] : 1.0f, min_p = A.p.min_p ? A.p.min_p[r] : 0.0f;
     const float uniform = A.uniform[r];
+    for (uint32_t i = tid; i < kBins; i += kThreads) {
+        s.mass[i] = 0;
+        s.count[i] = 0;
+    }
+    if (tid < 64) s.table[tid] = exp2(tid / 64.0);
+    if (tid == 0) {
+        s.n = 0;
+        s.kept_by_min = 0;
+    }
 
     // the largest logit (its lowest id) and the smallest finite one
-    float high = -__builtin_inff(), low = __builtin_inff();
+    float high = -kInf, low = kInf;
     uint32_t high_id = 0xffffffffu;
     bool bad = false;
     row.each([&](float x, uint32_t i) {
-        bad |= !(x < __builtin_inff());
-        if (x > high) {
-            high = x;
-            high_id = i;
-        }
-        if (x > -__builtin_inff()) low = fminf(low, x);
+        bad |= !(x < kInf);
+        high_id = x > high ? i : high_id;
+        high = fmaxf(high, x);
+        low = fminf(low, x > -kInf ? x : kInf);
     });
     for (uint32_t d = 32; d >= 1; d >>= 1) {
         const float h = __shfl_xor(high, d);
@@ -215,12 +412,8 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
         s.wave_id[wave] = high_id;
         s.wave_bad[wave] = bad;
     }
-    for (uint32_t i = tid; i < kBins; i += kThreads) {
-        s.mass[i] = 0;
-        s.count[i] = 0;
-    }
-    if (tid < 64) s.table[tid] = exp2(tid / 64.0);
     __syncthreads();
+#pragma unroll
     for (uint32_t i = 0; i < kWaves; ++i) {
         bad |= s.wave_bad[i];
         if (precedes(s.wave_a[i], s.wave_id[i], high, high_id)) {
@@ -229,8 +422,7 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
         }
         low = fminf(low, s.wave_b[i]);
     }
-    bad |= high == -__builtin_inff() || !(temperature >= 0.0f) || top_p != top_p || min_p != min_p ||
-           uniform != uniform;
+    bad |= high == -kInf || !(temperature >= 0.0f) || top_p != top_p || min_p != min_p || uniform != uniform;
     if (bad || temperature == 0.0f) {
         if (tid == 0) {
             A.ids[r] = bad ? 0xffffffffu : high_id;
@@ -239,226 +431,221 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
         }
         return;
     }
-    const double M = high, per_x = 1.4426950408889634 / static_cast<double>(temperature);
-    // log 2 of a weight; weights below 2^-46 are none
-    constexpr double kLeast = -46.0;
-    auto mass_of = [&](float x, double &w) -> uint64_t {
-        const double t = (static_cast<double>(x) - M) * per_x;
-        if (!(x > -__builtin_inff()) || !(t > kLeast)) return 0;
-        w = exp2_table(t, s.table);
-        // to an integer below 2^45 through the mantissa of 2^52 + it
-        return __builtin_bit_cast(uint64_t, w * 0x1p44 + 0x1p52) & 0xfffffffffffffull;
-    };
+    Weights w;
+    w.M = high;
+    w.M_d = high;
+    w.c = 1.4426950408889634 / static_cast<double>(temperature);
+    // (temperatures near 0, where a float does not hold the factor: all in double)
+    const bool small = w.c < 0x1p100;
+    w.c_hi = small ? static_cast<float>(w.c) : 0x1p100f;
+    w.c_lo = small ? static_cast<float>(w.c - static_cast<double>(w.c_hi)) : 0.0f;
+    w.heavy = !small ? -kInf : min_p > 0.0f ? fminf(-8.0f, __builtin_amdgcn_logf(min_p) - 0.125f) : -8.0f; // (log 2)
+    w.table = s.table;
+    const double reach = 46.0 / w.c, span = fmin(static_cast<double>(high) - static_cast<double>(low), reach);
+    const Steps steps{high, span > 0.0 ? static_cast<float>(fmin((kBins - 1) / span, 0x1p126)) : 0.0f};
+    const float u = fminf(fmaxf(uniform, 0.0f), 0x1.fffffep-1f);
 
-    // the histogram over the stretch that has weights, and min-p's mass
-    const double reach = -kLeast / per_x, span = fmin(M - static_cast<double>(low), reach);
-    const Steps steps{M, span > 0.0 ? (kBins - 1) / span : 0.0, kBins - 1};
-    uint64_t kept_m = 0;
-    row.each([&](float x, uint32_t) {
-        double w;
-        const uint64_t m = mass_of(x, w);
-        if (m == 0) return;
-        const uint32_t b = steps.of(x);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[b]), m);
-        atomicAdd(&s.count[b], 1u);
-        if (w >= static_cast<double>(min_p)) kept_m += m;
-    });
-    for (uint32_t d = 32; d >= 1; d >>= 1) kept_m += __shfl_xor(kept_m, d);
-    __syncthreads();
-    scan_bins(s, s.mass, s.count, kBins);
-    if (lane == 0) s.wave_mass[wave] = kept_m;
-    __syncthreads();
-    kept_m = 0;
-    for (uint32_t i = 0; i < kWaves; ++i) kept_m += s.wave_mass[i];
-    const uint64_t whole = s.mass[kBins - 1];
-    const uint32_t weighted = s.count[kBins - 1];
-
-    // The element at which `t` is first met: s.cut and the mass up to and with
-    // it, s.cut_mass. Every thread calls it, with a target that the last
-    // weighted element meets.
-    auto find = [&](const Target &t) {
-        __syncthreads();
-        for (uint32_t i = tid; i < kBins; i += kThreads)
-            if (t.met(s.count[i], s.mass[i]) && (i == 0 || !t.met(s.count[i - 1], s.mass[i - 1]))) s.step = i;
-        __syncthreads();
-        uint32_t step = s.step;
-        uint64_t m0 = step ? s.mass[step - 1] : 0;
-        uint32_t c0 = step ? s.count[step - 1] : 0, n = s.count[step] - c0;
-        // elements of the current stretch: those of all steps so far
-        float stretch_hi = high, stretch_lo = -__builtin_inff();
-        bool first = true;
-        auto inside = [&](float x) {
-            return first ? x > -__builtin_inff() && steps.of(x) == step : x <= stretch_hi && x >= stretch_lo;
-        };
-        while (n > kList) { // many elements: the stretch's own bounds, then finer steps
-            float a = -__builtin_inff(), b = __builtin_inff();
-            row.each([&](float x, uint32_t) {
-                double w;
-                if (inside(x) && mass_of(x, w)) {
-                    a = fmaxf(a, x);
-                    b = fminf(b, x);
-                }
-            });
-            for (uint32_t d = 32; d >= 1; d >>= 1) {
-                a = fmaxf(a, __shfl_xor(a, d));
-                b = fminf(b, __shfl_xor(b, d));
-            }
-            __syncthreads();
-            if (lane == 0) {
-                s.wave_a[wave] = a;
-                s.wave_b[wave] = b;
-            }
-            for (uint32_t i = tid; i < kFineBins; i += kThreads) {
-                s.fine_mass[i] = 0;
-                s.fine_count[i] = 0;
-            }
-            __syncthreads();
-            for (uint32_t i = 0; i < kWaves; ++i) {
-                a = fmaxf(a, s.wave_a[i]);
-                b = fminf(b, s.wave_b[i]);
-            }
-            if (a == b) { // equal logits: the r-th of them by id
-                double w;
-                const uint64_t m = mass_of(a, w);
-                uint32_t lo = 1, hi = n; // the least count that meets the target
-                while (lo < hi) {
-                    const uint32_t mid = (lo + hi) / 2;
-                    if (t.met(c0 + mid, m0 + mid * m)) hi = mid;
-                    else lo = mid + 1;
-                }
-                uint32_t left = lo;
-                for (uint32_t i0 = 0; i0 < V; i0 += kThreads) {
-                    const uint32_t i = i0 + tid;
-                    const bool here = i < V && row.from[i] == a;
-                    const uint64_t vote = __ballot(here);
-                    __syncthreads();
-                    if (lane == 0) s.wave_count[wave] = __builtin_popcountll(vote);
-                    __syncthreads();
-                    uint32_t before = 0, all = 0;
-                    for (uint32_t k = 0; k < kWaves; ++k) {
-                        before += k < wave ? s.wave_count[k] : 0;
-                        all += s.wave_count[k];
-                    }
-                    if (left > all) {
-                        left -= all;
-                        continue;
-                    }
-                    before += __builtin_popcountll(vote & ((uint64_t{1} << lane) - 1));
-                    if (here && before + 1 == left) {
-                        s.cut = Place{a, i};
-                        s.cut_mass = m0 + lo * m;
-                    }
-                    break;
-                }
-                __syncthreads();
-                return;
-            }
-            const Steps fine{static_cast<double>(a), (kFineBins - 1) / (static_cast<double>(a) - static_cast<double>(b)),
-                             kFineBins - 1};
-            row.each([&](float x, uint32_t) {
-                double w;
-                if (!inside(x)) return;
-                const uint64_t m = mass_of(x, w);
-                if (m == 0) return;
-                const uint32_t f = fine.of(x);
-                atomicAdd(reinterpret_cast<unsigned long long *>(&s.fine_mass[f]), m);
-                atomicAdd(&s.fine_count[f], 1u);
-            });
-            __syncthreads();
-            scan_bins(s, s.fine_mass, s.fine_count, kFineBins);
-            for (uint32_t i = tid; i < kFineBins; i += kThreads)
-                if (t.met(c0 + s.fine_count[i], m0 + s.fine_mass[i]) &&
-                    (i == 0 || !t.met(c0 + s.fine_count[i - 1], m0 + s.fine_mass[i - 1])))
-                    s.step = i;
-            __syncthreads();
-            const uint32_t f = s.step;
-            const uint64_t fm = f ? s.fine_mass[f - 1] : 0;
-            const uint32_t fc = f ? s.fine_count[f - 1] : 0;
-            n = s.fine_count[f] - fc;
-            m0 += fm;
-            c0 += fc;
-            // the elements of fine step f, as bounds on x
-            float na = -__builtin_inff(), nb = __builtin_inff();
-            row.each([&](float x, uint32_t) {
-                double w;
-                if (inside(x) && fine.of(x) == f && mass_of(x, w)) {
-                    na = fmaxf(na, x);
-                    nb = fminf(nb, x);
-                }
-            });
-            for (uint32_t d = 32; d >= 1; d >>= 1) {
-                na = fmaxf(na, __shfl_xor(na, d));
-                nb = fminf(nb, __shfl_xor(nb, d));
-            }
-            __syncthreads();
-            if (lane == 0) {
-                s.wave_a[wave] = na;
-                s.wave_b[wave] = nb;
-            }
-            __syncthreads();
-            for (uint32_t i = 0; i < kWaves; ++i) {
-                na = fmaxf(na, s.wave_a[i]);
-                nb = fminf(nb, s.wave_b[i]);
-            }
-            stretch_hi = na;
-            stretch_lo = nb;
-            first = false;
-        }
-        if (tid == 0) s.n = 0;
-        __syncthreads();
-        row.each([&](float x, uint32_t i) {
-            double w;
-            if (!inside(x)) return;
-            const uint64_t m = mass_of(x, w);
-            if (m == 0) return;
-            const uint32_t at = atomicAdd(&s.n, 1u);
-            if (at < kList) {
-                s.list_x[at] = x;
-                s.list_id[at] = i;
-                s.list_mass[at] = m;
-            }
+    // A small top-k: count, and list the steps down to the one that holds the
+    // k-th.
+    if (top_k != 0 && top_k <= kCountedTopK) {
+        row.each([&](float x, uint32_t) {
+            if (Weights::any(w.exponent(x))) atomicAdd(&s.count[steps.of(x)], 1u);
         });
         __syncthreads();
-        const uint32_t listed = s.n < kList ? s.n : kList;
-        if (tid < listed) {
-            const float x = s.list_x[tid];
-            const uint32_t id = s.list_id[tid];
-            uint64_t m = m0;
-            uint32_t c = c0;
-            for (uint32_t j = 0; j < listed; ++j)
-                if (precedes(s.list_x[j], s.list_id[j], x, id)) {
-                    m += s.list_mass[j];
-                    ++c;
-                }
-            const uint64_t with = m + s.list_mass[tid];
-            if (t.met(c + 1, with) && !t.met(c, m)) {
-                s.cut = Place{x, id};
-                s.cut_mass = with;
+        scan_steps(s); // (no masses)
+        const uint32_t weighted = s.count[kBins - 1], k = top_k < weighted ? top_k : weighted;
+        for (uint32_t i = tid; i < kBins; i += kThreads)
+            if (s.count[i] >= k && (i == 0 || s.count[i - 1] < k)) s.step = i;
+        __syncthreads();
+        const uint32_t step = s.step, listed = s.count[step];
+        if (listed <= kList) {
+            row.each([&](float x, uint32_t i) {
+                if (steps.of(x) <= step && Weights::any(w.exponent(x))) put(s, x, i);
+            });
+            __syncthreads();
+            // every element's predecessors: their number and mass
+            uint64_t m = 0, own = 0;
+            uint32_t c = 0, id = 0;
+            float x = 0.0f;
+            const bool mine = tid < listed;
+            double weight = 0.0;
+            if (mine) {
+                x = s.list_x[tid];
+                id = s.list_id[tid];
+                weight = w.exact(x);
+                own = w.of(x);
+                s.list_mass[tid] = own;
             }
+            __syncthreads();
+            if (mine)
+#pragma unroll 4
+                for (uint32_t j = 0; j < listed; ++j)
+                    if (precedes(s.list_x[j], s.list_id[j], x, id)) {
+                        m += s.list_mass[j];
+                        ++c;
+                    }
+            if (mine && c + 1 == k) s.cut_mass = m + own;
+            __syncthreads();
+            uint64_t kept = s.cut_mass;
+            const double reach_p = fmax(static_cast<double>(top_p) * static_cast<double>(kept), 1.0);
+            __syncthreads();
+            if (top_p < 1.0f) {
+                if (mine && static_cast<double>(m + own) >= reach_p && static_cast<double>(m) < reach_p) s.cut_mass = m + own;
+                __syncthreads();
+                kept = s.cut_mass < kept ? s.cut_mass : kept;
+            }
+            if (min_p > 0.0f) {
+                if (mine && weight >= static_cast<double>(min_p))
+                    atomicMax(reinterpret_cast<unsigned long long *>(&s.kept_by_min), m + own);
+                __syncthreads();
+                const uint64_t least = s.kept_by_min ? s.kept_by_min : uint64_t{1} << kMassBits; // the largest at least
+                kept = least < kept ? least : kept;
+            }
+            const double exceed = static_cast<double>(u) * static_cast<double>(kept);
+            if (mine && static_cast<double>(m + own) > exceed && !(static_cast<double>(m) > exceed)) {
+                A.ids[r] = id;
+                if (A.probs) A.probs[r] = static_cast<float>(weight * 0x1p44 / static_cast<double>(kept));
+            }
+            return;
+        }
+    }
+
+    // The steps' masses (and counts, for a large top-k), and the mass that min-p
+    // keeps. The heavy weights wait in the list, so that the others' code is
+    // short; where they are more than it takes, they come from a pass of their
+    // own.
+    const bool counted = top_k != 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < kBins; i += kThreads) s.count[i] = 0;
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    row.each([&](float x, uint32_t i) {
+        const float t = w.exponent(x);
+        if (!Weights::any(t)) return;
+        if (t >= w.heavy) {
+            put(s, x, i);
+            return;
+        }
+        const uint32_t b = steps.of(x);
+        atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[b]), w.light(t));
+        if (counted) atomicAdd(&s.count[b], 1u);
+    });
+    __syncthreads();
+    uint64_t by_min = 0;
+    const auto heavy = [&](float x) {
+        const double weight = w.exact(x);
+        const uint64_t m = Weights::mass(weight);
+        const uint32_t b = steps.of(x);
+        atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[b]), m);
+        if (counted) atomicAdd(&s.count[b], 1u);
+        if (weight >= static_cast<double>(min_p)) by_min += m;
+    };
+    const uint32_t heavies = s.n;
+    if (heavies <= kList) {
+        if (tid < heavies) heavy(s.list_x[tid]);
+    } else {
+        slow.each([&](float x, uint32_t) {
+            const float t = w.exponent(x);
+            if (Weights::any(t) && t >= w.heavy) heavy(x);
+        });
+    }
+    if (min_p > 0.0f && by_min) atomicAdd(reinterpret_cast<unsigned long long *>(&s.kept_by_min), by_min);
+    __syncthreads();
+    scan_steps(s);
+    uint64_t kept = s.mass[kBins - 1];
+    const uint64_t kept_by_min = s.kept_by_min;
+    const uint32_t weighted = s.count[kBins - 1];
+
+    // top-k, top-p and the choice itself, each a target that some element first
+    // meets
+    bool spoiled = false; // narrow() has taken the steps' arrays
+#pragma unroll 1
+    for (uint32_t stage = 0; stage < 3; ++stage) {
+        Target t;
+        if (stage == 0) {
+            if (!counted || top_k >= weighted) continue;
+            t = Target{kCount, top_k, 0.0};
+        } else if (stage == 1) {
+            if (!(top_p < 1.0f)) continue;
+            t = Target{kReach, 0, fmax(static_cast<double>(top_p) * static_cast<double>(kept), 1.0)};
+        } else {
+            if (min_p > 0.0f) {
+                const uint64_t least = kept_by_min ? kept_by_min : uint64_t{1} << kMassBits; // the largest at least
+                kept = least < kept ? least : kept;
+            }
+            t = Target{kExceed, 0, static_cast<double>(u) * static_cast<double>(kept)};
+        }
+        uint64_t m0 = 0;
+        uint32_t c0 = 0, step = 0;
+        float hi = high, lo = -kInf;
+        if (tid == 0) s.n = 0;
+        if (!spoiled) {
+            for (uint32_t i = tid; i < kBins; i += kThreads)
+                if (t.met(s.count[i], s.mass[i]) && (i == 0 || !t.met(s.count[i - 1], s.mass[i - 1]))) s.step = i;
+            __syncthreads();
+            step = s.step;
+            m0 = step ? s.mass[step - 1] : 0;
+            c0 = step && counted ? s.count[step - 1] : 0;
+            row.each([&](float x, uint32_t i) {
+                if (steps.of(x) == step && Weights::any(w.exponent(x))) put(s, x, i);
+            });
+        } else {
+            __syncthreads();
+            slow.each([&](float x, uint32_t i) {
+                if (Weights::any(w.exponent(x))) put(s, x, i);
+            });
         }
         __syncthreads();
-    };
-
-    uint64_t kept = whole;
-    if (top_k != 0 && top_k < weighted) {
-        find(Target{kCount, top_k, 0.0});
-        kept = s.cut_mass;
+        uint32_t n = s.n;
+        if (n > kList) {
+            if (!spoiled) { // the step's bounds
+                float a = -kInf, b = kInf;
+                slow.each([&](float x, uint32_t) {
+                    if (steps.of(x) == step && Weights::any(w.exponent(x))) {
+                        a = fmaxf(a, x);
+                        b = fminf(b, x);
+                    }
+                });
+                for (uint32_t d = 32; d >= 1; d >>= 1) {
+                    a = fmaxf(a, __shfl_xor(a, d));
+                    b = fminf(b, __shfl_xor(b, d));
+                }
+                if (lane == 0) {
+                    s.wave_a[wave] = a;
+                    s.wave_b[wave] = b;
+                }
+                __syncthreads();
+                for (uint32_t i = 0; i < kWaves; ++i) {
+                    a = fmaxf(a, s.wave_a[i]);
+                    b = fminf(b, s.wave_b[i]);
+                }
+                hi = a;
+                lo = b;
+            }
+            spoiled = true;
+            const bool found = narrow(s, slow, w, t, hi, lo, m0, c0, n);
+            if (found) {
+                if (stage < 2) kept = s.cut_mass < kept ? s.cut_mass : kept;
+                __syncthreads();
+                continue;
+            }
+            if (tid == 0) s.n = 0;
+            __syncthreads();
+            slow.each([&](float x, uint32_t i) {
+                if (x <= hi && x >= lo && Weights::any(w.exponent(x))) put(s, x, i);
+            });
+            __syncthreads();
+            n = s.n;
+        }
+        if (tid < n) s.list_mass[tid] = w.of(s.list_x[tid]);
+        __syncthreads();
+        rank_list(s, t, n, m0, c0);
+        if (stage < 2) kept = s.cut_mass < kept ? s.cut_mass : kept;
+        __syncthreads();
     }
-    if (top_p < 1.0f) {
-        find(Target{kReach, 0, fmax(static_cast<double>(top_p) * static_cast<double>(kept), 1.0)});
-        kept = s.cut_mass < kept ? s.cut_mass : kept;
-    }
-    if (min_p > 0.0f) {
-        const uint64_t least = kept_m ? kept_m : uint64_t{1} << kMassBits; // the largest at least
-        kept = least < kept ? least : kept;
-    }
-    const float u = fminf(fmaxf(uniform, 0.0f), 0x1.fffffep-1f);
-    find(Target{kExceed, 0, static_cast<double>(u) * static_cast<double>(kept)});
     if (tid == 0) {
-        double w = 0.0;
-        (void)mass_of(s.cut.x, w);
-        A.ids[r] = s.cut.id;
-        if (A.probs) A.probs[r] = static_cast<float>(w * 0x1p44 / static_cast<double>(kept));
+        A.ids[r] = s.cut_id;
+        if (A.probs) A.probs[r] = static_cast<float>(w.exact(s.cut_x) * 0x1p44 / static_cast<double>(kept));
     }
 }
 
@@ -469,7 +656,7 @@ uint64_t sample_scratch(uint32_t, uint32_t) { return 0; }
 int sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const fmx_sampling &p,
            const float *uniform, uint32_t *ids, float *probs, uint32_t *status, uint8_t *, hipStream_t s) {
     const SampleArgs A{logits, row_stride, vocab, p, uniform, ids, probs, status};
-    const auto kernel = vocab <= 8 * kThreads ? sample_kernel<8> : vocab <= 32 * kThreads ? sample_kernel<32> : sample_kernel<0>;
+    const auto kernel = vocab <= 8 * kThreads ? sample_kernel<8> : sample_kernel<0>;
     hipLaunchKernelGGL(kernel, dim3(rows), dim3(kThreads), 0, s, A);
     FMX_LAUNCH_CHECK();
     return FMX_OK;
