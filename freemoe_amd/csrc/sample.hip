@@ -9,8 +9,9 @@
 // exceeds uniform x that mass. Nothing is sorted: a place in the order where a
 // count or a mass crosses a target is found by a histogram over equal steps of
 // x, then among the elements of the one step that holds it, every one against
-// every other. A small top-k needs no masses but its own: the steps down to
-// the k-th logit are taken out at once.
+// every other. A small top-k needs no masses but its own: the k-th largest of
+// the threads' maxima bounds the k-th logit from below, and what lies above
+// that bound is listed in one pass.
 //
 // Masses are integers in steps of 2^-44: their sums do not depend on the order
 // of the additions (LDS atomics, whichever wavefront comes first).
@@ -20,16 +21,14 @@ namespace fmx {
 
 namespace {
 
-constexpr uint32_t kThreads = 1024;
-constexpr uint32_t kWaves = kThreads / 64;
+constexpr uint32_t kMaxWaves = 16;
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kList = 1024;  // elements compared pair by pair
+constexpr uint32_t kList = 512; // elements compared pair by pair
 constexpr uint32_t kMassBits = 44;
 static_assert(kSampleMaxVocab <= 1u << 18, "sums of that many masses of at most 2^44 stay below 2^63");
 
-// A top-k up to here is taken out by counts (the list holds it and the rest of
-// its last step).
-constexpr uint32_t kCountedTopK = 512;
+// A top-k up to here is listed through the threads' maxima.
+constexpr uint32_t kListedTopK = 256;
 
 struct SampleArgs {
     const float *logits;
@@ -91,8 +90,14 @@ struct Weights {
     }
 };
 
-__device__ __forceinline__ bool precedes(float xa, uint32_t ia, float xb, uint32_t ib) {
-    return xa > xb || (xa == xb && ia < ib);
+// An element's place in the order, as a number: falling logits, then rising ids.
+__device__ __forceinline__ uint64_t place_of(float x, uint32_t id) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f); // (-0 is 0)
+    return static_cast<uint64_t>(b >> 31 ? b : ~(b | 0x80000000u)) << 32 | id;
+}
+__device__ __forceinline__ float logit_of(uint64_t place) {
+    const uint32_t b = static_cast<uint32_t>(place >> 32);
+    return __builtin_bit_cast(float, b >> 31 ? b : ~b & 0x7fffffffu);
 }
 
 enum Mode : uint32_t { kCount, kReach, kExceed }; // count >= n; mass >= m; mass > m
@@ -107,21 +112,22 @@ struct Target {
     }
 };
 
+struct __align__(16) Listed {
+    uint64_t place, mass;
+};
+
 struct Shared {
-    uint64_t mass[kBins], list_mass[kList];
+    Listed list[kList];
+    uint64_t mass[kBins];
     uint32_t count[kBins];
-    float list_x[kList];
-    uint32_t list_id[kList];
     double table[64];
-    uint64_t wave_mass[kWaves];
-    uint32_t wave_count[kWaves];
-    float wave_a[kWaves], wave_b[kWaves];
-    uint32_t wave_id[kWaves];
-    bool wave_bad[kWaves];
+    uint64_t wave_mass[kMaxWaves];
+    uint32_t wave_count[kMaxWaves];
+    uint64_t wave_place[kMaxWaves];
+    float wave_a[kMaxWaves], wave_b[kMaxWaves];
+    bool wave_bad[kMaxWaves];
     uint32_t n, step;
-    float cut_x;
-    uint32_t cut_id;
-    uint64_t cut_mass, kept_by_min;
+    uint64_t cut_place, cut_mass, kept_by_min;
 };
 
 // Steps of x: element x lies in step floor((top - x) * scale), the last one
@@ -136,8 +142,8 @@ struct Steps {
 };
 
 // Inclusive sums of the steps' masses and counts, in place.
-__device__ __forceinline__ void scan_steps(Shared &s) {
-    constexpr uint32_t kPer = kBins / kThreads;
+template <uint32_t kThreads> __device__ __forceinline__ void scan_steps(Shared &s) {
+    constexpr uint32_t kPer = kBins / kThreads, kWaves = kThreads / 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t m[kPer], mi = 0;
     uint32_t c[kPer], ci = 0;
@@ -178,7 +184,7 @@ __device__ __forceinline__ void scan_steps(Shared &s) {
 }
 
 // The row in memory, one element at a time, for the passes few rows need.
-struct SlowRow {
+template <uint32_t kThreads> struct SlowRow {
     const float *from;
     uint32_t vocab;
     template <class F> __device__ __forceinline__ void each(const F &f) const {
@@ -187,67 +193,94 @@ struct SlowRow {
     }
 };
 
-// The row: kHeld elements a thread in registers, or (0) read again at each
-// pass, from L2.
-template <uint32_t kHeld> struct Row {
-    float held[kHeld ? kHeld : 1];
+// The row in 16-byte pieces, kAhead of a thread at a time, from memory at the
+// first pass and from L2 at the others (held in registers, 32000 elements a row
+// took 64 of them a thread and spilled): piece v holds elements 4 v - skew .. + 3,
+// skew being what the row's start lacks to the next lower multiple of 16 bytes.
+template <uint32_t kThreads> struct Row {
+    static constexpr uint32_t kAhead = 8;
     const float *from;
-    uint32_t vocab;
-    __device__ __forceinline__ void load() {
-        if constexpr (kHeld > 0)
-#pragma unroll
-            for (uint32_t r = 0; r < kHeld; ++r) {
-                const uint32_t i = r * kThreads + threadIdx.x;
-                held[r] = i < vocab ? from[i] : -__builtin_inff();
-            }
+    uint32_t vocab, skew, pieces;
+
+    __device__ __forceinline__ Row(const float *row, uint32_t n) : from(row), vocab(n) {
+        skew = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 2 & 3);
+        pieces = (skew + n + 3) / 4;
     }
-    template <class F> __device__ __forceinline__ void each(const F &f) const {
-        if constexpr (kHeld > 0) {
+    __device__ __forceinline__ void load(float (&x)[4 * kAhead], uint32_t v0) const {
 #pragma unroll
-            for (uint32_t r = 0; r < kHeld; ++r) f(held[r], r * kThreads + threadIdx.x);
-        } else {
-            constexpr uint32_t kAhead = 8;
-            for (uint32_t i0 = threadIdx.x; i0 < vocab; i0 += kAhead * kThreads) {
-                float x[kAhead];
+        for (uint32_t r = 0; r < kAhead; ++r) {
+            const uint32_t v = v0 + r * kThreads;
+            const int32_t i = static_cast<int32_t>(4 * v - skew);
 #pragma unroll
-                for (uint32_t r = 0; r < kAhead; ++r) {
-                    const uint32_t i = i0 + r * kThreads;
-                    x[r] = i < vocab ? from[i] : -__builtin_inff();
-                }
+            for (int j = 0; j < 4; ++j) x[4 * r + j] = -__builtin_inff();
+            if (v >= pieces) continue;
+            if (i >= 0 && i + 4 <= static_cast<int32_t>(vocab)) {
+                const uint4 w = ld16(from + i);
+                x[4 * r] = __builtin_bit_cast(float, w.x);
+                x[4 * r + 1] = __builtin_bit_cast(float, w.y);
+                x[4 * r + 2] = __builtin_bit_cast(float, w.z);
+                x[4 * r + 3] = __builtin_bit_cast(float, w.w);
+            } else {
 #pragma unroll
-                for (uint32_t r = 0; r < kAhead; ++r) f(x[r], i0 + r * kThreads);
+                for (int j = 0; j < 4; ++j)
+                    if (i + j >= 0 && i + j < static_cast<int32_t>(vocab)) x[4 * r + j] = from[i + j];
             }
+        }
+    }
+    // f(element, id), and -inf where a piece reaches past the row
+    template <class F> __device__ __forceinline__ void each(const F &f) const {
+        for (uint32_t v0 = threadIdx.x; v0 < pieces; v0 += kAhead * kThreads) {
+            float x[4 * kAhead];
+            load(x, v0);
+#pragma unroll
+            for (uint32_t r = 0; r < 4 * kAhead; ++r) f(x[r], 4 * (v0 + r / 4 * kThreads) + r % 4 - skew);
         }
     }
 };
 
 __device__ __forceinline__ void put(Shared &s, float x, uint32_t i) {
     const uint32_t at = atomicAdd(&s.n, 1u);
-    if (at < kList) {
-        s.list_x[at] = x;
-        s.list_id[at] = i;
+    if (at < kList) s.list[at].place = place_of(x, i);
+}
+
+// Number and mass of the listed elements before each: 2^k lanes next to each
+// other take an element's comparisons in turn, as many as the threads allow.
+// `e` is this thread's element (every lane of a group ends with its sums),
+// first whether it is the group's first lane.
+struct Before {
+    uint32_t e, count;
+    uint64_t mass;
+    bool first;
+};
+template <uint32_t kThreads> __device__ __forceinline__ Before count_before(Shared &s, uint32_t listed) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t lanes = 1;
+    while (lanes < 32 && listed * lanes * 2 <= kThreads) lanes *= 2;
+    Before b{tid / lanes, 0, 0, tid % lanes == 0 && tid / lanes < listed};
+    const uint64_t place = s.list[b.e < listed ? b.e : 0].place;
+#pragma unroll 4
+    for (uint32_t j = tid % lanes; j < listed; j += lanes) {
+        const Listed o = s.list[j];
+        const bool before = o.place < place;
+        b.mass += before ? o.mass : 0;
+        b.count += before;
     }
+    for (uint32_t d = 1; d < lanes; d <<= 1) {
+        b.mass += __shfl_xor(b.mass, d);
+        b.count += __shfl_xor(b.count, d);
+    }
+    return b;
 }
 
 // Of the listed elements, whose predecessors hold m0 and number c0: the one at
 // which `t` is first met, to s.cut_*.
+template <uint32_t kThreads>
 __device__ __forceinline__ void rank_list(Shared &s, const Target &t, uint32_t listed, uint64_t m0, uint32_t c0) {
-    const uint32_t tid = threadIdx.x;
-    if (tid < listed) {
-        const float x = s.list_x[tid];
-        const uint32_t id = s.list_id[tid];
-        uint64_t m = m0;
-        uint32_t c = c0;
-#pragma unroll 4
-        for (uint32_t j = 0; j < listed; ++j)
-            if (precedes(s.list_x[j], s.list_id[j], x, id)) {
-                m += s.list_mass[j];
-                ++c;
-            }
-        const uint64_t with = m + s.list_mass[tid];
-        if (t.met(c + 1, with) && !t.met(c, m)) {
-            s.cut_x = x;
-            s.cut_id = id;
+    const Before b = count_before<kThreads>(s, listed);
+    if (b.first) {
+        const uint64_t m = m0 + b.mass, with = m + s.list[b.e].mass;
+        if (t.met(c0 + b.count + 1, with) && !t.met(c0 + b.count, m)) {
+            s.cut_place = s.list[b.e].place;
             s.cut_mass = with;
         }
     }
@@ -258,8 +291,10 @@ __device__ __forceinline__ void rank_list(Shared &s, const Target &t, uint32_t l
 // <= x <= hi: narrowed by finer and finer steps, or, where all are equal,
 // counted off by id. Fills s.cut_* and returns true, or leaves the stretch's
 // bounds, mass and count for the list.
-__device__ __forceinline__ bool narrow(Shared &s, SlowRow row, Weights w, Target t, float &hi, float &lo, uint64_t &m0,
+template <uint32_t kThreads>
+__device__ __forceinline__ bool narrow(Shared &s, SlowRow<kThreads> row, Weights w, Target t, float &hi, float &lo, uint64_t &m0,
                                     uint32_t &c0, uint32_t &n) {
+    constexpr uint32_t kWaves = kThreads / 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     constexpr float kInf = __builtin_inff();
     // (the steps' sums have served; their arrays hold the finer ones)
@@ -317,8 +352,7 @@ __device__ __forceinline__ bool narrow(Shared &s, SlowRow row, Weights w, Target
                 }
                 before += __builtin_popcountll(vote & ((uint64_t{1} << lane) - 1));
                 if (here && before + 1 == left) {
-                    s.cut_x = a;
-                    s.cut_id = i;
+                    s.cut_place = place_of(a, i);
                     s.cut_mass = m0 + least * m;
                 }
                 break;
@@ -345,7 +379,7 @@ __device__ __forceinline__ bool narrow(Shared &s, SlowRow row, Weights w, Target
             atomicAdd(&s.count[f], 1u);
         });
         __syncthreads();
-        scan_steps(s);
+        scan_steps<kThreads>(s);
         for (uint32_t i = tid; i < kBins; i += kThreads)
             if (t.met(c0 + s.count[i], m0 + s.mass[i]) && (i == 0 || !t.met(c0 + s.count[i - 1], m0 + s.mass[i - 1])))
                 s.step = i;
@@ -363,15 +397,13 @@ __device__ __forceinline__ bool narrow(Shared &s, SlowRow row, Weights w, Target
 }
 
 // grid: rows.
-template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs A) {
+template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void sample_kernel(SampleArgs A) {
+    constexpr uint32_t kWaves = kThreads / 64;
     __shared__ Shared s;
     constexpr float kInf = __builtin_inff();
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x, V = A.vocab;
-    Row<kHeld> row;
-    row.from = A.logits + r * A.row_stride;
-    row.vocab = V;
-    row.load();
-    const SlowRow slow{row.from, V};
+    const Row<kThreads> row(A.logits + r * A.row_stride, V);
+    const SlowRow<kThreads> slow{row.from, V};
     const float temperature = A.p.temperature ? A.p.temperature[r] : 1.0f;
     const uint32_t top_k = A.p.top_k ? A.p.top_k[r] : 0;
     const float top_p = A.p.top_p ? A.p.top_p[r] : 1.0f, min_p = A.p.min_p ? A.p.min_p[r] : 0.0f;
@@ -386,48 +418,56 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
         s.kept_by_min = 0;
     }
 
-    // the largest logit (its lowest id) and the smallest finite one
+    // the largest and the smallest logit
     float high = -kInf, low = kInf;
-    uint32_t high_id = 0xffffffffu;
     bool bad = false;
-    row.each([&](float x, uint32_t i) {
-        bad |= !(x < kInf);
-        high_id = x > high ? i : high_id;
-        high = fmaxf(high, x);
-        low = fminf(low, x > -kInf ? x : kInf);
-    });
-    for (uint32_t d = 32; d >= 1; d >>= 1) {
-        const float h = __shfl_xor(high, d);
-        const uint32_t id = __shfl_xor(high_id, d);
-        if (precedes(h, id, high, high_id)) {
-            high = h;
-            high_id = id;
+    for (uint32_t v0 = tid; v0 < row.pieces; v0 += row.kAhead * kThreads) {
+        float x[4 * row.kAhead];
+        row.load(x, v0);
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * row.kAhead; i += 2) {
+            bad |= x[i] != x[i] || x[i + 1] != x[i + 1];
+            high = fmaxf(fmaxf(x[i], x[i + 1]), high);
+            low = fminf(fminf(x[i], x[i + 1]), low);
         }
+    }
+    const float own_high = high;
+    for (uint32_t d = 32; d >= 1; d >>= 1) {
+        high = fmaxf(high, __shfl_xor(high, d));
         low = fminf(low, __shfl_xor(low, d));
     }
     bad = __any(bad);
     if (lane == 0) {
         s.wave_a[wave] = high;
         s.wave_b[wave] = low;
-        s.wave_id[wave] = high_id;
         s.wave_bad[wave] = bad;
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < kWaves; ++i) {
         bad |= s.wave_bad[i];
-        if (precedes(s.wave_a[i], s.wave_id[i], high, high_id)) {
-            high = s.wave_a[i];
-            high_id = s.wave_id[i];
-        }
+        high = fmaxf(high, s.wave_a[i]);
         low = fminf(low, s.wave_b[i]);
     }
-    bad |= high == -kInf || !(temperature >= 0.0f) || top_p != top_p || min_p != min_p || uniform != uniform;
-    if (bad || temperature == 0.0f) {
+    bad |= !__builtin_isfinite(high) || !(temperature >= 0.0f) || top_p != top_p || min_p != min_p || uniform != uniform;
+    if (bad) {
         if (tid == 0) {
-            A.ids[r] = bad ? 0xffffffffu : high_id;
-            if (A.probs) A.probs[r] = bad ? 0.0f : 1.0f;
-            if (bad) atomicOr(A.status, STATUS_NONFINITE_SCORE);
+            A.ids[r] = 0xffffffffu;
+            if (A.probs) A.probs[r] = 0.0f;
+            atomicOr(A.status, STATUS_NONFINITE_SCORE);
+        }
+        return;
+    }
+    if (temperature == 0.0f) { // the lowest id of the largest
+        if (tid == 0) s.step = 0xffffffffu;
+        __syncthreads();
+        row.each([&](float x, uint32_t i) {
+            if (x == high) atomicMin(&s.step, i);
+        });
+        __syncthreads();
+        if (tid == 0) {
+            A.ids[r] = s.step;
+            if (A.probs) A.probs[r] = 1.0f;
         }
         return;
     }
@@ -441,69 +481,71 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
     w.c_lo = small ? static_cast<float>(w.c - static_cast<double>(w.c_hi)) : 0.0f;
     w.heavy = !small ? -kInf : min_p > 0.0f ? fminf(-8.0f, __builtin_amdgcn_logf(min_p) - 0.125f) : -8.0f; // (log 2)
     w.table = s.table;
-    const double reach = 46.0 / w.c, span = fmin(static_cast<double>(high) - static_cast<double>(low), reach);
+    const double reach = 46.0 / w.c, span = fmin(static_cast<double>(high) - static_cast<double>(low), reach); // (low: -inf too)
     const Steps steps{high, span > 0.0 ? static_cast<float>(fmin((kBins - 1) / span, 0x1p126)) : 0.0f};
     const float u = fminf(fmaxf(uniform, 0.0f), 0x1.fffffep-1f);
 
-    // A small top-k: count, and list the steps down to the one that holds the
-    // k-th.
-    if (top_k != 0 && top_k <= kCountedTopK) {
-        row.each([&](float x, uint32_t) {
-            if (Weights::any(w.exponent(x))) atomicAdd(&s.count[steps.of(x)], 1u);
+    // A small top-k: the k-th largest of the threads' maxima, or one a little
+    // below, bounds the k-th logit; what reaches it is listed. (Fewer than k
+    // threads with a weight: all that have one.)
+    if (top_k != 0 && top_k <= kListedTopK) {
+        const uint32_t own_step = steps.of(own_high);
+        const bool weighs = Weights::any(w.exponent(own_high));
+        if (weighs) atomicAdd(&s.count[own_step], 1u);
+        if (tid == 0) s.step = kBins - 1;
+        __syncthreads();
+        scan_steps<kThreads>(s); // (no masses)
+        for (uint32_t i = tid; i < kBins; i += kThreads)
+            if (s.count[i] >= top_k && (i == 0 || s.count[i - 1] < top_k)) s.step = i;
+        __syncthreads();
+        float least = -kInf;
+        if (s.count[kBins - 1] >= top_k) {
+            least = weighs && own_step <= s.step ? own_high : kInf;
+            for (uint32_t d = 32; d >= 1; d >>= 1) least = fminf(least, __shfl_xor(least, d));
+            if (lane == 0) s.wave_a[wave] = least;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < kWaves; ++i) least = fminf(least, s.wave_a[i]);
+        }
+        row.each([&](float x, uint32_t i) {
+            if (x >= least && Weights::any(w.exponent(x))) put(s, x, i);
         });
         __syncthreads();
-        scan_steps(s); // (no masses)
-        const uint32_t weighted = s.count[kBins - 1], k = top_k < weighted ? top_k : weighted;
-        for (uint32_t i = tid; i < kBins; i += kThreads)
-            if (s.count[i] >= k && (i == 0 || s.count[i - 1] < k)) s.step = i;
-        __syncthreads();
-        const uint32_t step = s.step, listed = s.count[step];
+        const uint32_t listed = s.n, k = top_k < listed ? top_k : listed;
         if (listed <= kList) {
-            row.each([&](float x, uint32_t i) {
-                if (steps.of(x) <= step && Weights::any(w.exponent(x))) put(s, x, i);
-            });
-            __syncthreads();
-            // every element's predecessors: their number and mass
-            uint64_t m = 0, own = 0;
-            uint32_t c = 0, id = 0;
-            float x = 0.0f;
-            const bool mine = tid < listed;
             double weight = 0.0;
-            if (mine) {
-                x = s.list_x[tid];
-                id = s.list_id[tid];
-                weight = w.exact(x);
-                own = w.of(x);
-                s.list_mass[tid] = own;
+            if (tid < listed) {
+                const float x = logit_of(s.list[tid].place);
+                s.list[tid].mass = w.of(x);
             }
             __syncthreads();
-            if (mine)
-#pragma unroll 4
-                for (uint32_t j = 0; j < listed; ++j)
-                    if (precedes(s.list_x[j], s.list_id[j], x, id)) {
-                        m += s.list_mass[j];
-                        ++c;
-                    }
-            if (mine && c + 1 == k) s.cut_mass = m + own;
+            const Before b = count_before<kThreads>(s, listed);
+            uint64_t with = 0;
+            bool mine = b.first && b.count < k;
+            if (mine) {
+                with = b.mass + s.list[b.e].mass;
+                weight = w.exact(logit_of(s.list[b.e].place));
+                if (b.count + 1 == k) s.cut_mass = with;
+            }
             __syncthreads();
             uint64_t kept = s.cut_mass;
-            const double reach_p = fmax(static_cast<double>(top_p) * static_cast<double>(kept), 1.0);
             __syncthreads();
             if (top_p < 1.0f) {
-                if (mine && static_cast<double>(m + own) >= reach_p && static_cast<double>(m) < reach_p) s.cut_mass = m + own;
+                const double least = fmax(static_cast<double>(top_p) * static_cast<double>(kept), 1.0);
+                if (mine && static_cast<double>(with) >= least && static_cast<double>(b.mass) < least) s.cut_mass = with;
                 __syncthreads();
                 kept = s.cut_mass < kept ? s.cut_mass : kept;
             }
             if (min_p > 0.0f) {
                 if (mine && weight >= static_cast<double>(min_p))
-                    atomicMax(reinterpret_cast<unsigned long long *>(&s.kept_by_min), m + own);
+                    atomicMax(reinterpret_cast<unsigned long long *>(&s.kept_by_min), with);
                 __syncthreads();
                 const uint64_t least = s.kept_by_min ? s.kept_by_min : uint64_t{1} << kMassBits; // the largest at least
                 kept = least < kept ? least : kept;
             }
             const double exceed = static_cast<double>(u) * static_cast<double>(kept);
-            if (mine && static_cast<double>(m + own) > exceed && !(static_cast<double>(m) > exceed)) {
-                A.ids[r] = id;
+            if (mine && static_cast<double>(with) > exceed && !(static_cast<double>(b.mass) > exceed)) {
+                A.ids[r] = static_cast<uint32_t>(s.list[b.e].place);
                 if (A.probs) A.probs[r] = static_cast<float>(weight * 0x1p44 / static_cast<double>(kept));
             }
             return;
@@ -542,7 +584,7 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
     };
     const uint32_t heavies = s.n;
     if (heavies <= kList) {
-        if (tid < heavies) heavy(s.list_x[tid]);
+        if (tid < heavies) heavy(logit_of(s.list[tid].place));
     } else {
         slow.each([&](float x, uint32_t) {
             const float t = w.exponent(x);
@@ -551,7 +593,7 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
     }
     if (min_p > 0.0f && by_min) atomicAdd(reinterpret_cast<unsigned long long *>(&s.kept_by_min), by_min);
     __syncthreads();
-    scan_steps(s);
+    scan_steps<kThreads>(s);
     uint64_t kept = s.mass[kBins - 1];
     const uint64_t kept_by_min = s.kept_by_min;
     const uint32_t weighted = s.count[kBins - 1];
@@ -637,15 +679,16 @@ template <uint32_t kHeld> __global__ __launch_bounds__(kThreads) void sample_ker
             __syncthreads();
             n = s.n;
         }
-        if (tid < n) s.list_mass[tid] = w.of(s.list_x[tid]);
+        if (tid < n) s.list[tid].mass = w.of(logit_of(s.list[tid].place));
         __syncthreads();
-        rank_list(s, t, n, m0, c0);
+        rank_list<kThreads>(s, t, n, m0, c0);
         if (stage < 2) kept = s.cut_mass < kept ? s.cut_mass : kept;
         __syncthreads();
     }
     if (tid == 0) {
-        A.ids[r] = s.cut_id;
-        if (A.probs) A.probs[r] = static_cast<float>(w.exact(s.cut_x) * 0x1p44 / static_cast<double>(kept));
+        A.ids[r] = static_cast<uint32_t>(s.cut_place);
+        if (A.probs)
+            A.probs[r] = static_cast<float>(w.exact(logit_of(s.cut_place)) * 0x1p44 / static_cast<double>(kept));
     }
 }
 
@@ -656,8 +699,12 @@ uint64_t sample_scratch(uint32_t, uint32_t) { return 0; }
 int sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const fmx_sampling &p,
            const float *uniform, uint32_t *ids, float *probs, uint32_t *status, uint8_t *, hipStream_t s) {
     const SampleArgs A{logits, row_stride, vocab, p, uniform, ids, probs, status};
-    const auto kernel = vocab <= 8 * kThreads ? sample_kernel<8> : sample_kernel<0>;
-    hipLaunchKernelGGL(kernel, dim3(rows), dim3(kThreads), 0, s, A);
+    // two workgroups of 512 a CU take turns at what few of their threads do;
+    // where rows leave CUs to themselves, one of 1024
+    if (rows >= 512)
+        hipLaunchKernelGGL(sample_kernel<512>, dim3(rows), dim3(512), 0, s, A);
+    else
+        hipLaunchKernelGGL(sample_kernel<1024>, dim3(rows), dim3(1024), 0, s, A);
     FMX_LAUNCH_CHECK();
     return FMX_OK;
 }
