@@ -23,7 +23,7 @@ namespace {
 
 constexpr uint32_t kMaxWaves = 16;
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kList = 512; // elements compared pair by pair
+constexpr uint32_t kList = 1024; // elements set aside; as many as a workgroup has threads are compared pair by pair
 constexpr uint32_t kMassBits = 44;
 static_assert(kSampleMaxVocab <= 1u << 18, "sums of that many masses of at most 2^44 stay below 2^63");
 
@@ -56,13 +56,14 @@ __device__ __forceinline__ double exp2_table(double t, const double *table) {
     return ldexp(fma(s * r, base, base), i >> 6);
 }
 
-// A row's weights. Those of at least 2^-8 of the largest, and all that min-p
-// might keep, come from double arithmetic; the others, a body that matters by
-// its sum, from v_exp_f32 on a product carried to 2^-24 of the exponent (about
-// 2^-20 of each weight, at most 2^-28 of the largest, in either direction).
-// Weights below 2^-46 are none.
+// A row's weights. Those of at least 1 / 8 of the largest, and those next to
+// min-p's border, come from double arithmetic ("heavy"); the others, a body
+// that matters by its sum, from v_exp_f32 on an exponent carried to 2^-24 of
+// itself (2^-20 of each weight, 2^-23 of the largest, in either direction, at
+// the very most). Weights below 2^-46 are none.
 struct Weights {
-    float M, c_hi, c_lo, heavy; // log 2 units per logit in two floats; exponents from `heavy` on in double
+    float M, c_hi, c_lo;    // log 2 units per logit in two floats
+    float heavy, border;    // exponents: from `heavy` on, and within 2^-10 of `border`, in double
     double M_d, c;
     const double *table;
 
@@ -72,9 +73,7 @@ struct Weights {
     }
     // d = -inf times a zero c is NaN: no weight, as any exponent not above -46
     static __device__ __forceinline__ bool any(float t) { return t > -46.0f; }
-    __device__ __forceinline__ uint64_t light(float t) const {
-        return static_cast<uint64_t>(static_cast<uint32_t>(fma_rn(__builtin_amdgcn_exp2f(t), 0x1p40f, 0.5f))) << 4;
-    }
+    __device__ __forceinline__ bool is_heavy(float t) const { return t >= heavy || fabsf(t - border) < 0x1p-10f; }
     __device__ __forceinline__ double exact(float x) const {
         const double t = (static_cast<double>(x) - M_d) * c;
         return t > -46.0 ? exp2_table(t, table) : 0.0;
@@ -83,10 +82,13 @@ struct Weights {
     static __device__ __forceinline__ uint64_t mass(double w) {
         return __builtin_bit_cast(uint64_t, w * 0x1p44 + 0x1p52) & 0xfffffffffffffull;
     }
+    static __device__ __forceinline__ uint64_t light(float t) {
+        return mass(static_cast<double>(__builtin_amdgcn_exp2f(t)));
+    }
     __device__ __forceinline__ uint64_t of(float x) const {
         const float t = exponent(x);
         if (!any(t)) return 0;
-        return t >= heavy ? mass(exact(x)) : light(t);
+        return is_heavy(t) ? mass(exact(x)) : light(t);
     }
 };
 
@@ -188,53 +190,74 @@ template <uint32_t kThreads> struct SlowRow {
     const float *from;
     uint32_t vocab;
     template <class F> __device__ __forceinline__ void each(const F &f) const {
+        float next = threadIdx.x < vocab ? from[threadIdx.x] : 0.0f;
 #pragma unroll 1
-        for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) f(from[i], i);
+        for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
+            const float x = next;
+            if (i + kThreads < vocab) next = from[i + kThreads];
+            f(x, i);
+        }
     }
 };
 
-// The row in 16-byte pieces, kAhead of a thread at a time, from memory at the
-// first pass and from L2 at the others (held in registers, 32000 elements a row
-// took 64 of them a thread and spilled): piece v holds elements 4 v - skew .. + 3,
-// skew being what the row's start lacks to the next lower multiple of 16 bytes.
-template <uint32_t kThreads> struct Row {
-    static constexpr uint32_t kAhead = 8;
+// The row, from memory at the first pass and from L2 at the others (held in
+// registers, 32000 elements took 64 of them a thread and spilled). kWide: in
+// 16-byte pieces, kAhead of a thread at a time: piece v holds elements 4 v -
+// skew .. + 3, skew being what the row's start lacks to the next lower multiple
+// of 16 bytes. Else an element at a time, so that a short row meets every
+// thread. A thread's elements come in batches of kBatch; -inf where one
+// reaches past the row.
+template <uint32_t kThreads, bool kWide> struct Row {
+    static constexpr uint32_t kAhead = 8, kBatch = kWide ? 4 * kAhead : 4;
     const float *from;
     uint32_t vocab, skew, pieces;
 
     __device__ __forceinline__ Row(const float *row, uint32_t n) : from(row), vocab(n) {
-        skew = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 2 & 3);
-        pieces = (skew + n + 3) / 4;
+        skew = kWide ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 2 & 3) : 0;
+        pieces = kWide ? (skew + n + 3) / 4 : n;
     }
-    __device__ __forceinline__ void load(float (&x)[4 * kAhead], uint32_t v0) const {
+    // element r of the batch whose first piece is v0
+    __device__ __forceinline__ uint32_t id(uint32_t v0, uint32_t r) const {
+        return kWide ? 4 * (v0 + r / 4 * kThreads) + r % 4 - skew : v0 + r * kThreads;
+    }
+    __device__ __forceinline__ void load(float (&x)[kBatch], uint32_t v0) const {
+        if constexpr (!kWide) {
 #pragma unroll
-        for (uint32_t r = 0; r < kAhead; ++r) {
-            const uint32_t v = v0 + r * kThreads;
-            const int32_t i = static_cast<int32_t>(4 * v - skew);
+            for (uint32_t r = 0; r < kBatch; ++r) x[r] = id(v0, r) < vocab ? from[id(v0, r)] : -__builtin_inff();
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[4 * r + j] = -__builtin_inff();
-            if (v >= pieces) continue;
-            if (i >= 0 && i + 4 <= static_cast<int32_t>(vocab)) {
-                const uint4 w = ld16(from + i);
-                x[4 * r] = __builtin_bit_cast(float, w.x);
-                x[4 * r + 1] = __builtin_bit_cast(float, w.y);
-                x[4 * r + 2] = __builtin_bit_cast(float, w.z);
-                x[4 * r + 3] = __builtin_bit_cast(float, w.w);
-            } else {
+            for (uint32_t r = 0; r < kAhead; ++r) {
+                const uint32_t v = v0 + r * kThreads;
+                const int32_t i = static_cast<int32_t>(4 * v - skew);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i + j >= 0 && i + j < static_cast<int32_t>(vocab)) x[4 * r + j] = from[i + j];
+                for (int j = 0; j < 4; ++j) x[4 * r + j] = -__builtin_inff();
+                if (v >= pieces) continue;
+                if (i >= 0 && i + 4 <= static_cast<int32_t>(vocab)) {
+                    const uint4 w = ld16(from + i);
+                    x[4 * r] = __builtin_bit_cast(float, w.x);
+                    x[4 * r + 1] = __builtin_bit_cast(float, w.y);
+                    x[4 * r + 2] = __builtin_bit_cast(float, w.z);
+                    x[4 * r + 3] = __builtin_bit_cast(float, w.w);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i + j >= 0 && i + j < static_cast<int32_t>(vocab)) x[4 * r + j] = from[i + j];
+                }
             }
         }
     }
-    // f(element, id), and -inf where a piece reaches past the row
-    template <class F> __device__ __forceinline__ void each(const F &f) const {
-        for (uint32_t v0 = threadIdx.x; v0 < pieces; v0 += kAhead * kThreads) {
-            float x[4 * kAhead];
+    template <class F> __device__ __forceinline__ void batches(const F &f) const { // f(elements, first piece)
+        for (uint32_t v0 = threadIdx.x; v0 < pieces; v0 += (kWide ? kAhead : kBatch) * kThreads) {
+            float x[kBatch];
             load(x, v0);
-#pragma unroll
-            for (uint32_t r = 0; r < 4 * kAhead; ++r) f(x[r], 4 * (v0 + r / 4 * kThreads) + r % 4 - skew);
+            f(x, v0);
         }
+    }
+    template <class F> __device__ __forceinline__ void each(const F &f) const { // f(element, id)
+        batches([&](const float (&x)[kBatch], uint32_t v0) {
+#pragma unroll
+            for (uint32_t r = 0; r < kBatch; ++r) f(x[r], id(v0, r));
+        });
     }
 };
 
@@ -322,7 +345,7 @@ __device__ __forceinline__ bool narrow(Shared &s, SlowRow<kThreads> row, Weights
             b = fminf(b, s.wave_b[i]);
         }
     };
-    while (n > kList) {
+    while (n > kThreads) {
         float a, b;
         bounds(a, b, [&](float x) { return x <= hi && x >= lo; });
         if (a == b) {
@@ -397,12 +420,12 @@ __device__ __forceinline__ bool narrow(Shared &s, SlowRow<kThreads> row, Weights
 }
 
 // grid: rows.
-template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void sample_kernel(SampleArgs A) {
+template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 4) void sample_kernel(SampleArgs A) {
     constexpr uint32_t kWaves = kThreads / 64;
     __shared__ Shared s;
     constexpr float kInf = __builtin_inff();
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x, V = A.vocab;
-    const Row<kThreads> row(A.logits + r * A.row_stride, V);
+    const Row<kThreads, kWide> row(A.logits + r * A.row_stride, V);
     const SlowRow<kThreads> slow{row.from, V};
     const float temperature = A.p.temperature ? A.p.temperature[r] : 1.0f;
     const uint32_t top_k = A.p.top_k ? A.p.top_k[r] : 0;
@@ -421,16 +444,14 @@ template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void samp
     // the largest and the smallest logit
     float high = -kInf, low = kInf;
     bool bad = false;
-    for (uint32_t v0 = tid; v0 < row.pieces; v0 += row.kAhead * kThreads) {
-        float x[4 * row.kAhead];
-        row.load(x, v0);
+    row.batches([&](const float (&x)[row.kBatch], uint32_t) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4 * row.kAhead; i += 2) {
+        for (uint32_t i = 0; i < row.kBatch; i += 2) {
             bad |= x[i] != x[i] || x[i + 1] != x[i + 1];
             high = fmaxf(fmaxf(x[i], x[i + 1]), high);
             low = fminf(fminf(x[i], x[i + 1]), low);
         }
-    }
+    });
     const float own_high = high;
     for (uint32_t d = 32; d >= 1; d >>= 1) {
         high = fmaxf(high, __shfl_xor(high, d));
@@ -479,7 +500,8 @@ template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void samp
     const bool small = w.c < 0x1p100;
     w.c_hi = small ? static_cast<float>(w.c) : 0x1p100f;
     w.c_lo = small ? static_cast<float>(w.c - static_cast<double>(w.c_hi)) : 0.0f;
-    w.heavy = !small ? -kInf : min_p > 0.0f ? fminf(-8.0f, __builtin_amdgcn_logf(min_p) - 0.125f) : -8.0f; // (log 2)
+    w.heavy = small ? -3.0f : -kInf;
+    w.border = min_p > 0.0f ? __builtin_amdgcn_logf(min_p) : kInf; // (log 2)
     w.table = s.table;
     const double reach = 46.0 / w.c, span = fmin(static_cast<double>(high) - static_cast<double>(low), reach); // (low: -inf too)
     const Steps steps{high, span > 0.0 ? static_cast<float>(fmin((kBins - 1) / span, 0x1p126)) : 0.0f};
@@ -512,7 +534,7 @@ template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void samp
         });
         __syncthreads();
         const uint32_t listed = s.n, k = top_k < listed ? top_k : listed;
-        if (listed <= kList) {
+        if (listed <= kThreads) {
             double weight = 0.0;
             if (tid < listed) {
                 const float x = logit_of(s.list[tid].place);
@@ -561,19 +583,21 @@ template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void samp
     for (uint32_t i = tid; i < kBins; i += kThreads) s.count[i] = 0;
     if (tid == 0) s.n = 0;
     __syncthreads();
+    uint64_t by_min = 0;
     row.each([&](float x, uint32_t i) {
         const float t = w.exponent(x);
         if (!Weights::any(t)) return;
-        if (t >= w.heavy) {
+        if (w.is_heavy(t)) {
             put(s, x, i);
             return;
         }
         const uint32_t b = steps.of(x);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[b]), w.light(t));
+        const uint64_t m = Weights::light(t);
+        atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[b]), m);
         if (counted) atomicAdd(&s.count[b], 1u);
+        if (t > w.border) by_min += m;
     });
     __syncthreads();
-    uint64_t by_min = 0;
     const auto heavy = [&](float x) {
         const double weight = w.exact(x);
         const uint64_t m = Weights::mass(weight);
@@ -584,11 +608,11 @@ template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void samp
     };
     const uint32_t heavies = s.n;
     if (heavies <= kList) {
-        if (tid < heavies) heavy(logit_of(s.list[tid].place));
+        for (uint32_t i = tid; i < heavies; i += kThreads) heavy(logit_of(s.list[i].place));
     } else {
         slow.each([&](float x, uint32_t) {
             const float t = w.exponent(x);
-            if (Weights::any(t) && t >= w.heavy) heavy(x);
+            if (Weights::any(t) && w.is_heavy(t)) heavy(x);
         });
     }
     if (min_p > 0.0f && by_min) atomicAdd(reinterpret_cast<unsigned long long *>(&s.kept_by_min), by_min);
@@ -639,7 +663,7 @@ template <uint32_t kThreads> __global__ __launch_bounds__(kThreads, 4) void samp
         }
         __syncthreads();
         uint32_t n = s.n;
-        if (n > kList) {
+        if (n > kThreads) {
             if (!spoiled) { // the step's bounds
                 float a = -kInf, b = kInf;
                 slow.each([&](float x, uint32_t) {
@@ -701,10 +725,11 @@ int sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t voc
     const SampleArgs A{logits, row_stride, vocab, p, uniform, ids, probs, status};
     // two workgroups of 512 a CU take turns at what few of their threads do;
     // where rows leave CUs to themselves, one of 1024
-    if (rows >= 512)
-        hipLaunchKernelGGL(sample_kernel<512>, dim3(rows), dim3(512), 0, s, A);
-    else
-        hipLaunchKernelGGL(sample_kernel<1024>, dim3(rows), dim3(1024), 0, s, A);
+    const uint32_t threads = rows >= 512 ? 512 : 1024;
+    const bool wide = vocab > 4 * threads;
+    const auto kernel = threads == 512 ? (wide ? sample_kernel<512, true> : sample_kernel<512, false>)
+                                       : (wide ? sample_kernel<1024, true> : sample_kernel<1024, false>);
+    hipLaunchKernelGGL(kernel, dim3(rows), dim3(threads), 0, s, A);
     FMX_LAUNCH_CHECK();
     return FMX_OK;
 }
