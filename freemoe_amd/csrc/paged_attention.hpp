@@ -381,12 +381,31 @@ template <int DP> struct Tile16<float, DP> {
 };
 
 // Scores from q . k, in units of 1 / per_score of log 2: q . k itself, or the
-// capped score.
+// capped score. Below 1 / 4, where scores mostly lie, the hyperbolic tangent is
+// its Taylor sum to x^9 (the next term is below 2^-26 of it), a fifth of
+// tanhf's instructions.
 template <class Scores> __device__ __forceinline__ void cap_scores(const AttentionArgs &A, Scores &s) {
     constexpr int kN = sizeof(Scores) / sizeof(float);
-    if (A.softcap != 0.0f)
+    if (A.softcap == 0.0f) return;
+    float most = 0.0f;
 #pragma unroll
-        for (int x = 0; x < kN; ++x) s[x] = tanhf(s[x] * A.scale) * A.softcap;
+    for (int x = 0; x < kN; ++x) {
+        s[x] *= A.scale;
+        most = fmaxf(most, fabsf(s[x])); // (a NaN is dropped here and kept by either form)
+    }
+    if (__any(most > 0.25f)) {
+#pragma unroll
+        for (int x = 0; x < kN; ++x) s[x] = tanhf(s[x]) * A.softcap;
+    } else {
+#pragma unroll
+        for (int x = 0; x < kN; ++x) {
+            const float q = s[x] * s[x];
+            float t = fma_rn(q, 62.0f / 2835.0f, -17.0f / 315.0f);
+            t = fma_rn(t, q, 2.0f / 15.0f);
+            t = fma_rn(t, q, -1.0f / 3.0f);
+            s[x] = fma_rn(t * q, s[x], s[x]) * A.softcap;
+        }
+    }
 }
 
 __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, uint32_t type, f32x4 x) {
@@ -1069,7 +1088,12 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs 
 // A split is worth its second launch and its sums' way through memory where
 // the tiles alone leave CUs idle; never into pieces below one unit of keys.
 constexpr uint32_t kFillRows = 2048, kFillTiles = 512; // workgroups that a split aims at
-constexpr uint32_t kRowsMost = 16; // rows of a sequence that the 16-row kernel takes
+// Rows of a sequence up to which the 16-row kernel takes a call. 32, 64 and 128
+// rows of 16 sequences over 4096 positions, 8 kv heads of 128, 16-row / 128-row
+// kernel, us: bf16 80 / 57, 126 / 59, 211 / 71; f32 160 / 226, 268 / 407, 485 /
+// 420 (an f32 block takes a wavefront's 32 rows as long as its 128-row tile's
+// idle wavefronts wait for it; in 16 bits the keys' way to the CU counts).
+constexpr uint32_t rows_most(uint32_t type) { return type == FMX_TYPE_F32 ? 64 : 16; }
 
 // Scratch of a split call: stats, then sums.
 struct Scratch {
@@ -1114,7 +1138,7 @@ struct Plan {
 };
 Plan plan_of(const PagedArgs &a, uint32_t type, uint32_t group) {
     Plan p;
-    const bool rows = static_cast<uint64_t>(a.max_new) * group <= kRowsMost;
+    const bool rows = static_cast<uint64_t>(a.max_new) * group <= rows_most(type);
     p.tile_rows = rows ? kRows : kTileRows;
     p.unit = rows ? (type == FMX_TYPE_F32 ? 16 : 32) * kWaves
                   : kBlock;

@@ -176,6 +176,20 @@ ATTENTION = {
     "peaked": (4, 2, 128, BF16, F32, 16, [5, 70], [300, 70], dict(peak=6.0)),
     "peaked_f16": (4, 2, 128, F16, F32, 16, [5, 70], [300, 70], dict(peak=6.0)),
     "more_tokens_than_positions": (2, 1, 64, BF16, F32, 16, [5, 3], [2, 0], {}),
+    "softcap_wide": (4, 2, 64, F32, F32, 16, [3, 80], [90, 130], dict(softcap=50.0)),
+    # pages that split a load's rows, and every width the prompt kernels compute at
+    "prompt_pages_of_1": (4, 2, 128, BF16, BF16, 1, [70, 40], [130, 41], {}),
+    "prompt_pages_of_5": (2, 1, 64, F16, F32, 5, [150], [333], {}),
+    "prompt_pages_of_6_wide": (2, 1, 256, BF16, F32, 6, [70], [97], {}),
+    "prompt_pages_of_12_wide": (2, 1, 248, F16, F16, 12, [70, 64], [97, 64], {}),
+    "prompt_88": (3, 3, 88, BF16, F32, 24, [65, 66], [100, 66], dict(window=64)),
+    "prompt_112": (2, 1, 112, F16, F16, 16, [129], [129], {}),
+    "prompt_f32_wide": (2, 2, 200, F32, F32, 16, [129, 30], [140, 31], {}),
+    "prompt_f32_pages_of_7": (1, 1, 128, F32, F32, 7, [129], [200], {}),
+    "prompt_f32_64": (2, 1, 64, F32, F32, 16, [90], [300], {}),
+    "split_tiles": (2, 1, 64, BF16, F32, 16, [70], [4100], {}),
+    "split_tiles_f32": (1, 1, 32, F32, F32, 16, [70], [2100], dict(window=1999)),
+    "one_row_of_a_tile_more": (1, 1, 128, BF16, BF16, 16, [129, 257], [129, 300], {}),
     "negative_scale": (4, 2, 64, BF16, F32, 16, [1, 70], [90, 70], dict(scale=-0.2)),
     "no_scale": (4, 2, 64, F16, F32, 16, [1, 70], [90, 70], dict(scale=0.0)),
     "rising_scores": (2, 1, 64, F16, F32, 16, [3, 40], [700, 400], dict(rise=True)),
@@ -303,6 +317,66 @@ def test_attention_paged_reports_what_it_does_not_follow(gpu):
     assert run(lambda P: None) == (0, True, True)
     for change in (page, long, many):
         assert run(change) == (1, True, True)
+
+
+@pytest.mark.parametrize("dtype,out", [(BF16, F32), (F16, F16), (F32, F32)])
+def test_attention_paged_long(gpu, dtype, out):
+    """Long sequences, whose keys go to hundreds of workgroups, beside short ones,
+    single tokens and a chunk, against float64 on the GPU."""
+    H, G, D, ps = 4, 2, 64, 16
+    for counts, lengths in (([1, 1, 1], [70000, 5, 33001]), ([1, 40, 2], [20000, 30011, 17])):
+        P = ref.Paged(counts, lengths, G, D, ps, dtype, 53)
+        q = torch.randn(P.tokens, H, D, generator=P.g).to(dtype)
+        cache, batch = P.on(gpu)
+        got = torch.full((P.tokens, H, D), 7.0, dtype=out, device=gpu)
+        ws = sv.attention_workspace(cache, batch, H)
+        sv.attention(cache, batch, q.to(gpu), got, ws)
+        assert sv.status(ws) == 0
+        for i, (n, length) in enumerate(zip(counts, lengths)):
+            k, v = (P.rows(i, w).to(gpu).double() for w in (0, 1))
+            rows = slice(P.starts[i], P.starts[i] + n)
+            hidden = torch.arange(length, device=gpu) > length - n + torch.arange(n, device=gpu)[:, None]
+            for h in range(H):
+                kk, vv, qq = k[:, h // (H // G)], v[:, h // (H // G)], q[rows, h].to(gpu).double()
+                p = torch.softmax((qq @ kk.t() / math.sqrt(D)).masked_fill(hidden, -math.inf), 1)
+                want, spread = p @ vv, p @ vv.abs()
+                size = (qq.abs() @ kk.abs().t()).amax(1, keepdim=True) / math.sqrt(D)
+                # (the sums of the n weights lie in pieces of at most 2000, joined in f32)
+                weight = 2 * U * (D + 8) * size + U * (2000 + 600) + (0 if out == F32 else ref.bound_of(out))
+                tol = weight * spread + ref.half_step(out, want.abs() + weight * spread)
+                assert ((got[rows, h].double() - want).abs() <= tol).all(), (i, h)
+
+
+def test_attention_paged_one_workspace_for_two_captures(gpu):
+    """Two captured calls of different shapes that share a workspace, replayed one
+    after the other in both orders."""
+    calls = []
+    need = 0
+    for i, (counts, lengths) in enumerate((([1, 1], [3000, 100]), ([50], [1300]))):
+        P = ref.Paged(counts, lengths, 2, 64, 16, BF16, 60 + i)
+        cache, batch = P.on(gpu)
+        q = torch.randn(P.tokens, 8, 64, generator=P.g).to(BF16).to(gpu)
+        need = max(need, sv.attention_workspace(cache, batch, 8).numel())
+        calls.append((cache, batch, q, torch.zeros(P.tokens, 8, 64, device=gpu)))
+    ws = sv.workspace(need, gpu)
+    wants, graphs = [], []
+    for cache, batch, q, out in calls:
+        sv.attention(cache, batch, q, out, ws)
+        torch.cuda.synchronize()
+        wants.append(out.clone())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            sv.attention(cache, batch, q, out, ws)
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for c in calls:
+            c[3].zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for c, want in zip(calls, wants):
+            assert torch.equal(c[3], want), order
+    assert sv.status(ws) == 0
 
 
 def test_attention_paged_beyond_32_bit_offsets(gpu):
