@@ -60,13 +60,17 @@ __device__ __forceinline__ uint64_t position_offset(const PagedArgs &a, uint32_t
     return static_cast<uint64_t>(off ? 0 : page) * a.page_bytes + static_cast<uint64_t>(place) * a.position_bytes;
 }
 
-__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(v, d);
-        v += lane >= d ? o : 0;
-    }
-    return v;
+// Inclusive sums over the wavefront by DPP moves: within rows of 16 lanes, then
+// each row's last sum into the rows behind it.
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    int x = static_cast<int>(v);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false); // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); // row_bcast:31 into rows 2 and 3
+    return static_cast<uint32_t>(x);
 }
 
 // Item `target` of the batch where sequence i holds per(sequence) items: the
@@ -83,7 +87,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs &a, uint32_t target, c
         if (i < a.sequences) mine = sequence_at(a, i);
         bad |= __any(mine.bad);
         const uint32_t n = per(mine);
-        const uint32_t incl = wave_scan_u32(n, lane);
+        const uint32_t incl = wave_scan_u32(n);
         const uint64_t hit = __ballot(incl > target);
         if (hit) {
             const int at = __builtin_ctzll(hit);

@@ -143,28 +143,28 @@ struct Steps {
     }
 };
 
-// Inclusive sums of the steps' masses and counts, in place.
-template <uint32_t kThreads> __device__ __forceinline__ void scan_steps(Shared &s) {
+// Inclusive sums of the steps' counts and, kMasses, masses, in place.
+template <uint32_t kThreads, bool kMasses = true> __device__ __forceinline__ void scan_steps(Shared &s) {
     constexpr uint32_t kPer = kBins / kThreads, kWaves = kThreads / 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t m[kPer], mi = 0;
     uint32_t c[kPer], ci = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) {
-        mi += s.mass[tid * kPer + i];
+        if (kMasses) mi += s.mass[tid * kPer + i];
         ci += s.count[tid * kPer + i];
         m[i] = mi;
         c[i] = ci;
     }
     const uint64_t own_m = mi;
     const uint32_t own_c = ci;
+    ci = wave_scan_u32(ci);
+    if (kMasses)
 #pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint64_t mo = __shfl_up(mi, d);
-        const uint32_t co = __shfl_up(ci, d);
-        mi += lane >= d ? mo : 0;
-        ci += lane >= d ? co : 0;
-    }
+        for (uint32_t d = 1; d < 64; d <<= 1) {
+            const uint64_t mo = __shfl_up(mi, d);
+            mi += lane >= d ? mo : 0;
+        }
     if (lane == 63) {
         s.wave_mass[wave] = mi;
         s.wave_count[wave] = ci;
@@ -174,12 +174,12 @@ template <uint32_t kThreads> __device__ __forceinline__ void scan_steps(Shared &
     ci -= own_c;
 #pragma unroll
     for (uint32_t i = 0; i < kWaves; ++i) {
-        mi += i < wave ? s.wave_mass[i] : 0;
+        if (kMasses) mi += i < wave ? s.wave_mass[i] : 0;
         ci += i < wave ? s.wave_count[i] : 0;
     }
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) {
-        s.mass[tid * kPer + i] = mi + m[i];
+        if (kMasses) s.mass[tid * kPer + i] = mi + m[i];
         s.count[tid * kPer + i] = ci + c[i];
     }
     __syncthreads();
@@ -516,7 +516,7 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
         if (weighs) atomicAdd(&s.count[own_step], 1u);
         if (tid == 0) s.step = kBins - 1;
         __syncthreads();
-        scan_steps<kThreads>(s); // (no masses)
+        scan_steps<kThreads, false>(s);
         for (uint32_t i = tid; i < kBins; i += kThreads)
             if (s.count[i] >= top_k && (i == 0 || s.count[i - 1] < top_k)) s.step = i;
         __syncthreads();

@@ -178,8 +178,10 @@ def ptr(t) -> int:
 
 def stream_handle(stream=None) -> int:
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # (the handle without a Stream object around it: 4 us less per call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def packed_bytes(type_id: int, rows: int, cols: int) -> int:
