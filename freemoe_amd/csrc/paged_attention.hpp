@@ -422,7 +422,9 @@ __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, uint32_t type, 
 
 // Four elements of a row's sums with their maximum and the sum of weights: to
 // the output, with the sink's weight and divided, or, of a split tile, to where
-// attention_join_kernel takes them up.
+// attention_join_kernel takes them up. A row at a position before the first sees
+// nothing and is zero; any other sees itself, and without a score above -inf
+// (NaN, or -inf alone) its sums make it NaN, as they should.
 __device__ __forceinline__ void finish(const AttentionArgs &A, const Job &job, uint32_t tile_rows, uint32_t r,
                                        uint32_t head, uint32_t token, uint32_t d, float top, float mass, f32x4 o,
                                        float lift) {
@@ -433,14 +435,15 @@ __device__ __forceinline__ void finish(const AttentionArgs &A, const Job &job, u
         if (d == 0) A.stats[at] = make_float2(top, mass);
         return;
     }
-    if (A.sinks && top != kNegInf) {
+    const bool sees = job.before + static_cast<int32_t>(token - job.start) >= 0;
+    if (A.sinks && sees) {
         const float sink = A.sinks[head] * 0x1.715476p+0f; // log2 e
         const float best = fmaxf(top, sink), f = exp2_fast(top - best);
         mass = mass * f + exp2_fast(sink - best + lift);
         o *= f;
     }
-    if (top == kNegInf) o = f32x4{};
-    else o /= mass;
+    if (sees) o /= mass;
+    else o = f32x4{};
     const uint32_t size = A.out_type == FMX_TYPE_F32 ? 4 : 2;
     store4(A.out + token * A.out_bytes + static_cast<uint64_t>(head) * D * size, d, A.out_type, o);
 }
@@ -1044,6 +1047,7 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs 
     const uint32_t rows = seq.count * G;
     job.r0 = item * tile_rows;
     job.r1 = job.r0 + tile_rows < rows ? job.r0 + tile_rows : rows;
+    job.start = seq.start;
     job.before = static_cast<int32_t>(seq.length) - static_cast<int32_t>(seq.count);
     visible_keys(A, job.before, job.r0, job.r1, job.lo, job.hi);
     const uint32_t count = pieces_of(job.hi - job.lo, A.splits, unit).count;

@@ -406,8 +406,9 @@ typedef struct fmx_attention_options {
  * type), out_stride apart. Strides are multiples of 16 bytes, pointers 16-byte
  * aligned. A token that sees nothing (more new tokens than positions) gets
  * zeros. What a token does not see does not reach it, NaN and infinities there
- * included; of those it does see, a score makes its row NaN and an element of a
- * value that element of its row not finite. Scores and softmax statistics are
+ * included; of those it does see, a score of NaN or +inf makes its row NaN (one
+ * of -inf has no weight, and where all have none and there is no sink the row is
+ * NaN), and an element of a value that element of its row not finite. Scores and softmax statistics are
  * f32. An f32 result carries f32 accuracy whatever the cache's
  * type; for a 16-bit one the weights are rounded to 16 bits before they meet
  * the values. max_new chooses the kernel: state it as it is. */

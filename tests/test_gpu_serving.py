@@ -291,6 +291,36 @@ def test_attention_paged_unseen_values_stay_out(gpu, dtype, counts, window):
         assert rest.all() if sees else not rest.any(), r
 
 
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("counts,lengths", [([1, 1], [1, 5]), ([1, 2], [3000, 9]), ([150, 40], [150, 3000])])
+def test_attention_paged_scores_that_are_no_numbers(gpu, counts, lengths, dtype, sinks):
+    """Sequence 0 sees nothing but scores of NaN, or of -inf: its rows are NaN, as a
+    softmax over those is; a sink beside -inf alone takes all the weight. Sequence
+    1 keeps its values."""
+    H, G, D = 4, 2, 80
+    P = ref.Paged(counts, lengths, G, D, 16, dtype, 6)
+    cache, batch = P.on(gpu)
+    q = torch.rand(P.tokens, H, D, generator=P.g).add_(0.5).to(dtype).to(gpu)
+    sink = torch.zeros(H, device=gpu) if sinks else None
+    ws = sv.attention_workspace(cache, batch, H)
+    out = torch.empty(P.tokens, H, D, dtype=F32, device=gpu)
+    sv.attention(cache, batch, q, out, ws, sinks=sink)
+    want = out.cpu()[counts[0]:P.starts[-1]]
+    assert torch.isfinite(want).all()
+    mine = torch.tensor(P.pages[0], device=gpu)
+    for value in (math.nan, -math.inf):
+        cache.k[mine] = value
+        sv.attention(cache, batch, q, out, ws, sinks=sink)
+        got = out.cpu()
+        if sinks and value < 0:
+            assert (got[:counts[0]] == 0).all()
+        else:
+            assert torch.isnan(got[:counts[0]]).all()
+        assert torch.equal(got[counts[0]:P.starts[-1]], want)
+    assert sv.status(ws) == 0
+
+
 def test_attention_paged_reports_what_it_does_not_follow(gpu):
     def run(change):
         P = ref.Paged([1, 2, 1], [40, 30, 20], 1, 32, 8, F32, 29)
