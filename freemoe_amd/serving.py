@@ -72,15 +72,28 @@ class Rope:
         self.inv_freq = torch.tensor(list(inv), dtype=torch.float64, device=device)
         self.layout, self.dims, self.magnitude = layout, dims, magnitude.value
 
-    def desc(self, positions=None):
-        return fmx.Rope(self.layout, self.dims, self.inv_freq.data_ptr(), self.magnitude, fmx.ptr(positions) or None)
+    def desc(self, positions=None):  # positions: a device address
+        return fmx.Rope(self.layout, self.dims, self.inv_freq.data_ptr(), self.magnitude, positions)
 
 
-def _rows(t: torch.Tensor, tokens: int) -> int:
+def _rows(t: torch.Tensor, tokens: int, heads: int, head_dim: int, dtype=None) -> int:
     """Row stride of [tokens, heads, head_dim] (the heads of a row next to each other)."""
-    if t.dim() != 3 or t.shape[0] < tokens or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    n, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    if n < tokens or h != heads or d != head_dim or s2 != 1 or (h > 1 and s1 != d):
         raise ValueError("rows: [tokens, heads, head_dim], a row's heads next to each other")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"rows of {dtype}, not {t.dtype}")
+    return s0 if n > 1 else max(s0, h * d)
+
+
+def _entries(t: torch.Tensor | None, count: int, dtype):
+    """A device array of `count` entries, or NULL."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() < count or not t.is_contiguous():
+        raise ValueError(f"an array of {count} entries of {dtype}, next to each other")
+    return t.data_ptr()
 
 
 def workspace(bytes_: int = 256, device="cuda") -> torch.Tensor:
@@ -93,9 +106,11 @@ def status(ws: torch.Tensor, stream=None) -> int:
 
 
 def rope_append(cache: Cache, batch: Batch, rope: Rope, q, k, v, q_out, ws, positions=None, stream=None):
-    fmx.call("fmx_rope_append", ctypes.byref(cache.desc), ctypes.byref(batch.desc), ctypes.byref(rope.desc(positions)),
-             q.shape[1], TYPE_IDS[q.dtype], q.data_ptr(), _rows(q, batch.tokens), k.data_ptr(), _rows(k, batch.tokens),
-             v.data_ptr(), _rows(v, batch.tokens), q_out.data_ptr(), _rows(q_out, batch.tokens), ws.data_ptr(),
+    n, heads, kv_heads, d, dtype = batch.tokens, q.shape[1], cache.desc.kv_heads, cache.desc.head_dim, q.dtype
+    fmx.call("fmx_rope_append", ctypes.byref(cache.desc), ctypes.byref(batch.desc),
+             ctypes.byref(rope.desc(_entries(positions, n, torch.int32))), heads, TYPE_IDS[dtype], q.data_ptr(),
+             _rows(q, n, heads, d), k.data_ptr(), _rows(k, n, kv_heads, d, dtype), v.data_ptr(),
+             _rows(v, n, kv_heads, d, dtype), q_out.data_ptr(), _rows(q_out, n, heads, d, cache.k.dtype), ws.data_ptr(),
              ws.numel(), fmx.stream_handle(stream))
     return q_out
 
@@ -108,11 +123,12 @@ def attention_workspace(cache: Cache, batch: Batch, heads: int) -> torch.Tensor:
 
 
 def attention(cache: Cache, batch: Batch, q, out, ws, scale=None, softcap=0.0, window=0, sinks=None, stream=None):
-    options = fmx.AttentionOptions(1.0 / math.sqrt(q.shape[2]) if scale is None else scale, softcap, window,
-                                   fmx.ptr(sinks) or None)
-    fmx.call("fmx_attention_paged", ctypes.byref(cache.desc), ctypes.byref(batch.desc), ctypes.byref(options), q.shape[1],
-             q.data_ptr(), _rows(q, batch.tokens), TYPE_IDS[out.dtype], out.data_ptr(), _rows(out, batch.tokens),
-             ws.data_ptr(), ws.numel(), fmx.stream_handle(stream))
+    n, heads, d = batch.tokens, q.shape[1], cache.desc.head_dim
+    options = fmx.AttentionOptions(1.0 / math.sqrt(d) if scale is None else scale, softcap, window,
+                                   _entries(sinks, heads, torch.float32))
+    fmx.call("fmx_attention_paged", ctypes.byref(cache.desc), ctypes.byref(batch.desc), ctypes.byref(options), heads,
+             q.data_ptr(), _rows(q, n, heads, d, cache.k.dtype), TYPE_IDS[out.dtype], out.data_ptr(),
+             _rows(out, n, heads, d), ws.data_ptr(), ws.numel(), fmx.stream_handle(stream))
     return out
 
 
@@ -120,13 +136,15 @@ def sample(logits, uniform, ws=None, temperature=None, top_k=None, top_p=None, m
            stream=None):
     """Token ids (int32) and their probabilities, one per row of logits."""
     rows, vocab = logits.shape
-    if logits.dtype != torch.float32 or logits.stride(1) != 1:
+    if logits.dtype != torch.float32 or (vocab > 1 and logits.stride(1) != 1):
         raise ValueError("logits: float32 rows")
     ids = torch.empty(rows, dtype=torch.int32, device=logits.device) if ids is None else ids
     probs = torch.empty(rows, dtype=torch.float32, device=logits.device) if probs is None else probs
     ws = workspace(fmx.lib().fmx_sample_workspace_bytes(rows, vocab), logits.device) if ws is None else ws
-    settings = fmx.Sampling(*(fmx.ptr(t) or None for t in (temperature, top_k, top_p, min_p)))
+    f32 = torch.float32
+    settings = fmx.Sampling(_entries(temperature, rows, f32), _entries(top_k, rows, torch.int32),
+                            _entries(top_p, rows, f32), _entries(min_p, rows, f32))
     fmx.call("fmx_sample", logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-             ctypes.byref(settings), uniform.data_ptr(), ids.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(),
-             fmx.stream_handle(stream))
+             ctypes.byref(settings), _entries(uniform, rows, f32), _entries(ids, rows, torch.int32),
+             _entries(probs, rows, f32), ws.data_ptr(), ws.numel(), fmx.stream_handle(stream))
     return ids, probs

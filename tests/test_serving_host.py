@@ -10,6 +10,7 @@ import torch
 
 import serving_ref as ref
 from freemoe_amd import fmx
+from freemoe_amd import serving as sv
 
 
 def buffer():
@@ -111,6 +112,37 @@ def test_sample_refusals():
     assert sample(settings=None) == 1 and sample(ws=None) == 1 and sample(ws=p + 4) == 1 and sample(ws_bytes=255) == 1
     assert sample(rows=0) == 0
     assert lib.fmx_sample_workspace_bytes(1, 100) >= 256
+
+
+def test_tensors_that_do_not_fit_are_refused():
+    """The tensors' types and shapes, before an address reaches the library."""
+    bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
+    cache = sv.Cache(2, 16, 2, 64, bf16, "cpu")
+    batch = sv.Batch(torch.tensor([0, 2], dtype=i32), torch.tensor([5], dtype=i32), torch.zeros(1, 2, dtype=i32), 2, 2)
+    rope, ws = sv.Rope(64, device="cpu"), sv.workspace(device="cpu")
+    rows = lambda heads, dtype, tokens=2, dim=64: torch.zeros(tokens, heads, dim, dtype=dtype)
+    for q, out, more in [(rows(4, f32), rows(4, f32), {}), (rows(4, bf16, 1), rows(4, bf16), {}),
+                         (rows(4, bf16, dim=32), rows(4, bf16), {}), (rows(4, bf16), rows(2, bf16), {}),
+                         (rows(8, bf16)[:, ::2], rows(4, bf16), {}), (rows(4, bf16, dim=128)[..., ::2], rows(4, bf16), {}),
+                         (rows(4, bf16), rows(4, bf16), dict(sinks=torch.zeros(3))),
+                         (rows(4, bf16), rows(4, bf16), dict(sinks=torch.zeros(4, dtype=bf16)))]:
+        with pytest.raises(ValueError):
+            sv.attention(cache, batch, q, out, ws, **more)
+    for q, k, v, out, more in [(rows(4, f32), rows(2, bf16), rows(2, f32), rows(4, bf16), {}),
+                               (rows(4, f32), rows(2, f32), rows(2, bf16), rows(4, bf16), {}),
+                               (rows(4, f32), rows(2, f32), rows(2, f32), rows(4, f32), {}),
+                               (rows(4, f32), rows(4, f32), rows(2, f32), rows(4, bf16), {}),
+                               (rows(4, f32), rows(2, f32), rows(2, f32, 1), rows(4, bf16), {}),
+                               (rows(4, f32), rows(2, f32), rows(2, f32), rows(4, bf16), dict(positions=torch.zeros(2, dtype=torch.int64))),
+                               (rows(4, f32), rows(2, f32), rows(2, f32), rows(4, bf16), dict(positions=torch.zeros(1, dtype=i32)))]:
+        with pytest.raises(ValueError):
+            sv.rope_append(cache, batch, rope, q, k, v, out, ws, **more)
+    x, u = torch.zeros(3, 10), torch.zeros(3)
+    for logits, uniform, more in [(x.half(), u, {}), (torch.zeros(3, 20)[:, ::2], u, {}), (x, u[:2], {}), (x, u.double(), {}),
+                                  (x, torch.zeros(6)[::2], {}), (x, u, dict(top_k=torch.zeros(3))),
+                                  (x, u, dict(temperature=torch.zeros(1))), (x, u, dict(ids=torch.zeros(3, dtype=torch.int64)))]:
+        with pytest.raises(ValueError):
+            sv.sample(logits, uniform, ws, **more)
 
 
 def frequencies(dims, *scaling):
