@@ -56,14 +56,14 @@ __device__ __forceinline__ double exp2_table(double t, const double *table) {
     return ldexp(fma(s * r, base, base), i >> 6);
 }
 
-// A row's weights. Those of at least 1 / 8 of the largest, and those next to
-// min-p's border, come from double arithmetic ("heavy"); the others, a body
+// A row's weights. Those of about 1 / 8 of the largest and more, and those next
+// to min-p's border, come from double arithmetic ("heavy"); the others, a body
 // that matters by its sum, from v_exp_f32 on an exponent carried to 2^-24 of
 // itself (2^-20 of each weight, 2^-23 of the largest, in either direction, at
 // the very most). Weights below 2^-46 are none.
 struct Weights {
-    float M, c_hi, c_lo;    // log 2 units per logit in two floats
-    float heavy, border;    // exponents: from `heavy` on, and within 2^-10 of `border`, in double
+    float M, c_hi, c_lo;          // log 2 units per logit in two floats
+    float heavy, border, passed;  // logits: from `heavy` on, and `border` to `passed` (2^-10 around it), in double
     double M_d, c;
     const double *table;
 
@@ -73,14 +73,14 @@ struct Weights {
     }
     // d = -inf times a zero c is NaN: no weight, as any exponent not above -46
     static __device__ __forceinline__ bool any(float t) { return t > -46.0f; }
-    __device__ __forceinline__ bool is_heavy(float t) const { return t >= heavy || fabsf(t - border) < 0x1p-10f; }
+    __device__ __forceinline__ bool is_heavy(float x) const { return x >= heavy || (x >= border && x <= passed); }
     __device__ __forceinline__ double exact(float x) const {
         const double t = (static_cast<double>(x) - M_d) * c;
         return t > -46.0 ? exp2_table(t, table) : 0.0;
     }
     // an integer below 2^45 through the mantissa of 2^52 + it
     static __device__ __forceinline__ uint64_t mass(double w) {
-        return __builtin_bit_cast(uint64_t, w * 0x1p44 + 0x1p52) & 0xfffffffffffffull;
+        return __builtin_bit_cast(uint64_t, fma(w, 0x1p44, 0x1p52)) & 0xfffffffffffffull;
     }
     static __device__ __forceinline__ uint64_t light(float t) {
         return mass(static_cast<double>(__builtin_amdgcn_exp2f(t)));
@@ -88,7 +88,7 @@ struct Weights {
     __device__ __forceinline__ uint64_t of(float x) const {
         const float t = exponent(x);
         if (!any(t)) return 0;
-        return is_heavy(t) ? mass(exact(x)) : light(t);
+        return is_heavy(x) ? mass(exact(x)) : light(t);
     }
 };
 
@@ -119,29 +119,51 @@ struct __align__(16) Listed {
 };
 
 struct Shared {
-    Listed list[kList];
+    Listed list[kList], few[kList];
     uint64_t mass[kBins];
     uint32_t count[kBins];
     double table[64];
     uint64_t wave_mass[kMaxWaves];
     uint32_t wave_count[kMaxWaves];
-    uint64_t wave_place[kMaxWaves];
     float wave_a[kMaxWaves], wave_b[kMaxWaves];
     bool wave_bad[kMaxWaves];
-    uint32_t n, step;
+    uint64_t part_mass[64];
+    uint32_t part_count[64];
+    uint32_t n, n2, step;
     uint64_t cut_place, cut_mass, kept_by_min;
 };
 
 // Steps of x: element x lies in step floor((top - x) * scale), the last one
 // taking the rest; monotonic in x, so the steps are stretches of the order.
-// (An infinite difference at an infinite temperature: scale 0, step 0.)
+// (An infinite difference at an infinite temperature: the last, without a weight.)
 struct Steps {
     float top, scale;
     __device__ __forceinline__ uint32_t of(float x) const {
         const float d = (top - x) * scale;
-        return d < static_cast<float>(kBins - 1) ? static_cast<uint32_t>(d) : d > 0.0f ? kBins - 1 : 0;
+        return static_cast<uint32_t>(fminf(d, kBins - 1)); // (a NaN: the last)
+    }
+    // A step's 64 parts.
+    __device__ __forceinline__ uint32_t part(float x, uint32_t step) const {
+        const float d = ((top - x) * scale - static_cast<float>(step)) * 64.0f;
+        return static_cast<uint32_t>(fminf(fmaxf(d, 0.0f), 63.0f));
+    }
+    // Logits outside [lo, hi] are not in the step: d above comes to within 2^-22
+    // of itself, and a bound rounded to the nearest float passes no float by.
+    __device__ __forceinline__ void reach(uint32_t step, float &lo, float &hi) const {
+        const double of = scale, t = top;
+        lo = scale == 0.0f || step == kBins - 1 ? -__builtin_inff()
+                                                : static_cast<float>(t - (step + 1) * (1.0 + 0x1p-20) / of);
+        hi = scale == 0.0f || step == 0 ? __builtin_inff() : static_cast<float>(t - step * (1.0 - 0x1p-20) / of);
     }
 };
+
+// Inclusive sums over the wavefront, of numbers below 2^63 whose sum is.
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+    constexpr uint32_t k21 = (1u << 21) - 1;
+    const uint64_t a = wave_scan_u32(static_cast<uint32_t>(v) & k21), b = wave_scan_u32(static_cast<uint32_t>(v >> 21) & k21),
+                   c = wave_scan_u32(static_cast<uint32_t>(v >> 42));
+    return a + (b << 21) + (c << 42);
+}
 
 // Inclusive sums of the steps' counts and, kMasses, masses, in place.
 template <uint32_t kThreads, bool kMasses = true> __device__ __forceinline__ void scan_steps(Shared &s) {
@@ -159,12 +181,7 @@ template <uint32_t kThreads, bool kMasses = true> __device__ __forceinline__ voi
     const uint64_t own_m = mi;
     const uint32_t own_c = ci;
     ci = wave_scan_u32(ci);
-    if (kMasses)
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint64_t mo = __shfl_up(mi, d);
-            mi += lane >= d ? mo : 0;
-        }
+    if (kMasses) mi = wave_scan_u64(mi);
     if (lane == 63) {
         s.wave_mass[wave] = mi;
         s.wave_count[wave] = ci;
@@ -201,14 +218,15 @@ template <uint32_t kThreads> struct SlowRow {
 };
 
 // The row, from memory at the first pass and from L2 at the others (held in
-// registers, 32000 elements took 64 of them a thread and spilled). kWide: in
-// 16-byte pieces, kAhead of a thread at a time: piece v holds elements 4 v -
+// registers, 32 elements a thread, one row of 32000 took 17 us for 12). kWide:
+// in 16-byte pieces, kAhead of a thread at a time: piece v holds elements 4 v -
 // skew .. + 3, skew being what the row's start lacks to the next lower multiple
 // of 16 bytes. Else an element at a time, so that a short row meets every
 // thread. A thread's elements come in batches of kBatch; -inf where one
 // reaches past the row.
 template <uint32_t kThreads, bool kWide> struct Row {
     static constexpr uint32_t kAhead = 8, kBatch = kWide ? 4 * kAhead : 4;
+    static constexpr uint32_t kPieces = (kWide ? kAhead : kBatch) * kThreads; // of a batch, all threads
     const float *from;
     uint32_t vocab, skew, pieces;
 
@@ -216,47 +234,62 @@ template <uint32_t kThreads, bool kWide> struct Row {
         skew = kWide ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 2 & 3) : 0;
         pieces = kWide ? (skew + n + 3) / 4 : n;
     }
-    // element r of the batch whose first piece is v0
-    __device__ __forceinline__ uint32_t id(uint32_t v0, uint32_t r) const {
+    // element r of this thread's batch whose first pieces are b0 on
+    __device__ __forceinline__ uint32_t id(uint32_t b0, uint32_t r) const {
+        const uint32_t v0 = b0 + threadIdx.x;
         return kWide ? 4 * (v0 + r / 4 * kThreads) + r % 4 - skew : v0 + r * kThreads;
     }
-    __device__ __forceinline__ void load(float (&x)[kBatch], uint32_t v0) const {
+    __device__ __forceinline__ void load(float (&x)[kBatch], uint32_t b0) const {
         if constexpr (!kWide) {
 #pragma unroll
-            for (uint32_t r = 0; r < kBatch; ++r) x[r] = id(v0, r) < vocab ? from[id(v0, r)] : -__builtin_inff();
+            for (uint32_t r = 0; r < kBatch; ++r) x[r] = id(b0, r) < vocab ? from[id(b0, r)] : -__builtin_inff();
         } else {
+            const float *const base = from - skew + 4 * static_cast<uint64_t>(b0 + threadIdx.x);
 #pragma unroll
             for (uint32_t r = 0; r < kAhead; ++r) {
-                const uint32_t v = v0 + r * kThreads;
-                const int32_t i = static_cast<int32_t>(4 * v - skew);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[4 * r + j] = -__builtin_inff();
-                if (v >= pieces) continue;
-                if (i >= 0 && i + 4 <= static_cast<int32_t>(vocab)) {
-                    const uint4 w = ld16(from + i);
+                const uint32_t v = b0 + r * kThreads; // the workgroup's first piece
+                if ((v != 0 || skew == 0) && 4 * (v + kThreads) - skew <= vocab) {
+                    const uint4 w = ld16(base + 4 * r * kThreads);
                     x[4 * r] = __builtin_bit_cast(float, w.x);
                     x[4 * r + 1] = __builtin_bit_cast(float, w.y);
                     x[4 * r + 2] = __builtin_bit_cast(float, w.z);
                     x[4 * r + 3] = __builtin_bit_cast(float, w.w);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (i + j >= 0 && i + j < static_cast<int32_t>(vocab)) x[4 * r + j] = from[i + j];
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t i = id(b0, 4 * r + j); // (below 0: a large number)
+                        x[4 * r + j] = i < vocab ? from[i] : -__builtin_inff();
+                    }
                 }
             }
         }
     }
     template <class F> __device__ __forceinline__ void batches(const F &f) const { // f(elements, first piece)
-        for (uint32_t v0 = threadIdx.x; v0 < pieces; v0 += (kWide ? kAhead : kBatch) * kThreads) {
+        for (uint32_t b0 = 0; b0 < pieces; b0 += kPieces) {
             float x[kBatch];
-            load(x, v0);
-            f(x, v0);
+            load(x, b0);
+            f(x, b0);
         }
     }
-    template <class F> __device__ __forceinline__ void each(const F &f) const { // f(element, id)
-        batches([&](const float (&x)[kBatch], uint32_t v0) {
+    // f(element, id) for those from lo to hi: few, so four at a time are passed over
+    template <class F> __device__ __forceinline__ void between(float lo, float hi, const F &f) const {
+        batches([&](const float (&x)[kBatch], uint32_t b0) {
 #pragma unroll
-            for (uint32_t r = 0; r < kBatch; ++r) f(x[r], id(v0, r));
+            for (uint32_t r = 0; r < kBatch; r += 4) {
+                bool in[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) in[j] = x[r + j] >= lo && x[r + j] <= hi;
+                if (!(in[0] || in[1] || in[2] || in[3])) continue;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    if (in[j]) f(x[r + j], id(b0, r + j));
+            }
+        });
+    }
+    template <class F> __device__ __forceinline__ void each(const F &f) const { // f(element, id)
+        batches([&](const float (&x)[kBatch], uint32_t b0) {
+#pragma unroll
+            for (uint32_t r = 0; r < kBatch; ++r) f(x[r], id(b0, r));
         });
     }
 };
@@ -266,48 +299,62 @@ __device__ __forceinline__ void put(Shared &s, float x, uint32_t i) {
     if (at < kList) s.list[at].place = place_of(x, i);
 }
 
-// Number and mass of the listed elements before each: 2^k lanes next to each
-// other take an element's comparisons in turn, as many as the threads allow.
-// `e` is this thread's element (every lane of a group ends with its sums),
-// first whether it is the group's first lane.
-struct Before {
-    uint32_t e, count;
-    uint64_t mass;
-    bool first;
-};
-template <uint32_t kThreads> __device__ __forceinline__ Before count_before(Shared &s, uint32_t listed) {
+// Of the listed elements, whose predecessors hold m0 and number c0: the one at
+// which `t` is first met, to s.cut_*. Each against every other, 2^k lanes next
+// to each other taking an element's comparisons in turn, as many as the threads
+// allow.
+template <uint32_t kThreads>
+__device__ __forceinline__ void rank_list(Shared &s, const Listed *list, const Target &t, uint32_t listed, uint64_t m0,
+                                          uint32_t c0) {
     const uint32_t tid = threadIdx.x;
     uint32_t lanes = 1;
     while (lanes < 32 && listed * lanes * 2 <= kThreads) lanes *= 2;
-    Before b{tid / lanes, 0, 0, tid % lanes == 0 && tid / lanes < listed};
-    const uint64_t place = s.list[b.e < listed ? b.e : 0].place;
+    const uint32_t e = tid / lanes;
+    const uint64_t place = list[e < listed ? e : 0].place;
+    uint64_t m = 0;
+    uint32_t c = 0;
 #pragma unroll 4
     for (uint32_t j = tid % lanes; j < listed; j += lanes) {
-        const Listed o = s.list[j];
+        const Listed o = list[j];
         const bool before = o.place < place;
-        b.mass += before ? o.mass : 0;
-        b.count += before;
+        m += before ? o.mass : 0;
+        c += before;
     }
     for (uint32_t d = 1; d < lanes; d <<= 1) {
-        b.mass += __shfl_xor(b.mass, d);
-        b.count += __shfl_xor(b.count, d);
+        m += __shfl_xor(m, d);
+        c += __shfl_xor(c, d);
     }
-    return b;
-}
-
-// Of the listed elements, whose predecessors hold m0 and number c0: the one at
-// which `t` is first met, to s.cut_*.
-template <uint32_t kThreads>
-__device__ __forceinline__ void rank_list(Shared &s, const Target &t, uint32_t listed, uint64_t m0, uint32_t c0) {
-    const Before b = count_before<kThreads>(s, listed);
-    if (b.first) {
-        const uint64_t m = m0 + b.mass, with = m + s.list[b.e].mass;
-        if (t.met(c0 + b.count + 1, with) && !t.met(c0 + b.count, m)) {
-            s.cut_place = s.list[b.e].place;
+    if (tid % lanes == 0 && e < listed) {
+        const uint64_t with = m0 + m + list[e].mass;
+        if (t.met(c0 + c + 1, with) && !t.met(c0 + c, m0 + m)) {
+            s.cut_place = list[e].place;
             s.cut_mass = with;
         }
     }
     __syncthreads();
+}
+
+// The same for a step's elements: the part of the step that meets the target
+// first, then that part's few. (s.part_* and s.n2 are 0.)
+template <uint32_t kThreads>
+__device__ __forceinline__ void rank_step(Shared &s, const Steps &steps, uint32_t step, const Target &t, uint32_t listed,
+                                          uint64_t m0, uint32_t c0) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t part = tid < listed ? steps.part(logit_of(s.list[tid].place), step) : 64;
+    if (tid < listed) {
+        atomicAdd(reinterpret_cast<unsigned long long *>(&s.part_mass[part]), s.list[tid].mass);
+        atomicAdd(&s.part_count[part], 1u);
+    }
+    __syncthreads();
+    const uint64_t own = s.part_mass[lane];
+    const uint32_t own_c = s.part_count[lane];
+    const uint64_t m = m0 + wave_scan_u64(own);
+    const uint32_t c = c0 + wave_scan_u32(own_c);
+    const uint64_t met = __ballot(t.met(c, m));
+    const int at = met ? __builtin_ctzll(met) : 63;
+    if (part == static_cast<uint32_t>(at)) s.few[atomicAdd(&s.n2, 1u)] = s.list[tid];
+    __syncthreads();
+    rank_list<kThreads>(s, s.few, t, s.n2, __shfl(m - own, at), __shfl(c - own_c, at));
 }
 
 // A stretch of the order with more elements than the list takes, those with lo
@@ -500,8 +547,13 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
     const bool small = w.c < 0x1p100;
     w.c_hi = small ? static_cast<float>(w.c) : 0x1p100f;
     w.c_lo = small ? static_cast<float>(w.c - static_cast<double>(w.c_hi)) : 0.0f;
-    w.heavy = small ? -3.0f : -kInf;
-    w.border = min_p > 0.0f ? __builtin_amdgcn_logf(min_p) : kInf; // (log 2)
+    w.heavy = small ? static_cast<float>(w.M_d - 3.0 / w.c) : -kInf;
+    w.border = w.passed = kInf;
+    if (min_p > 0.0f) {
+        const double at = __builtin_amdgcn_logf(min_p); // (log 2)
+        w.border = static_cast<float>(w.M_d + (at - 0x1p-10) / w.c);
+        w.passed = static_cast<float>(w.M_d + (at + 0x1p-10) / w.c);
+    }
     w.table = s.table;
     const double reach = 46.0 / w.c, span = fmin(static_cast<double>(high) - static_cast<double>(low), reach); // (low: -inf too)
     const Steps steps{high, span > 0.0 ? static_cast<float>(fmin((kBins - 1) / span, 0x1p126)) : 0.0f};
@@ -520,41 +572,62 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
         for (uint32_t i = tid; i < kBins; i += kThreads)
             if (s.count[i] >= top_k && (i == 0 || s.count[i - 1] < top_k)) s.step = i;
         __syncthreads();
-        float least = -kInf;
-        if (s.count[kBins - 1] >= top_k) {
-            least = weighs && own_step <= s.step ? own_high : kInf;
-            for (uint32_t d = 32; d >= 1; d >>= 1) least = fminf(least, __shfl_xor(least, d));
-            if (lane == 0) s.wave_a[wave] = least;
-            __syncthreads();
+        const bool enough = s.count[kBins - 1] >= top_k;
+        float least = weighs && own_step <= s.step ? own_high : kInf;
+        for (uint32_t d = 32; d >= 1; d >>= 1) least = fminf(least, __shfl_xor(least, d));
+        if (lane == 0) s.wave_a[wave] = least;
+        __syncthreads();
+        for (uint32_t i = tid; i < kBins; i += kThreads) s.count[i] = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < kWaves; ++i) least = fminf(least, s.wave_a[i]);
-        }
-        row.each([&](float x, uint32_t i) {
-            if (x >= least && Weights::any(w.exponent(x))) put(s, x, i);
+        for (uint32_t i = 0; i < kWaves; ++i) least = fminf(least, s.wave_a[i]);
+        __syncthreads();
+        row.between(enough ? least : -kInf, kInf, [&](float x, uint32_t i) {
+            if (!Weights::any(w.exponent(x))) return;
+            const uint32_t at = atomicAdd(&s.n, 1u);
+            if (at < kThreads) s.list[at] = Listed{place_of(x, i), atomicAdd(&s.count[steps.of(x)], 1u)};
         });
         __syncthreads();
         const uint32_t listed = s.n, k = top_k < listed ? top_k : listed;
         if (listed <= kThreads) {
-            double weight = 0.0;
+            // sorted: by steps, each element's number within its step having come
+            // with the count, then within a step against its few others
+            scan_steps<kThreads, false>(s);
+            uint64_t place = 0, own = 0, with = 0;
+            uint32_t rank = 0, end = 0;
             if (tid < listed) {
-                const float x = logit_of(s.list[tid].place);
-                s.list[tid].mass = w.of(x);
+                place = s.list[tid].place;
+                const float x = logit_of(place);
+                const uint32_t step = steps.of(x);
+                own = w.of(x);
+                rank = step ? s.count[step - 1] : 0;
+                end = s.count[step];
+                s.few[rank + s.list[tid].mass].place = place;
             }
             __syncthreads();
-            const Before b = count_before<kThreads>(s, listed);
-            uint64_t with = 0;
-            bool mine = b.first && b.count < k;
-            if (mine) {
-                with = b.mass + s.list[b.e].mass;
-                weight = w.exact(logit_of(s.list[b.e].place));
-                if (b.count + 1 == k) s.cut_mass = with;
+            if (tid < listed) {
+                uint32_t to = rank;
+                for (uint32_t j = rank; j < end; ++j) to += s.few[j].place < place;
+                s.list[to] = Listed{place, own};
             }
+            __syncthreads();
+            double weight = 0.0;
+            own = tid < listed ? s.list[tid].mass : 0;
+            place = tid < listed ? s.list[tid].place : 0;
+            with = wave_scan_u64(own);
+            if (lane == 63) s.wave_mass[wave] = with;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < kWaves; ++i) with += i < wave ? s.wave_mass[i] : 0;
+            const uint64_t before = with - own;
+            const bool mine = tid < k;
+            if (mine) weight = w.exact(logit_of(place));
+            if (tid + 1 == k) s.cut_mass = with;
             __syncthreads();
             uint64_t kept = s.cut_mass;
             __syncthreads();
             if (top_p < 1.0f) {
                 const double least = fmax(static_cast<double>(top_p) * static_cast<double>(kept), 1.0);
-                if (mine && static_cast<double>(with) >= least && static_cast<double>(b.mass) < least) s.cut_mass = with;
+                if (mine && static_cast<double>(with) >= least && static_cast<double>(before) < least) s.cut_mass = with;
                 __syncthreads();
                 kept = s.cut_mass < kept ? s.cut_mass : kept;
             }
@@ -566,8 +639,8 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
                 kept = least < kept ? least : kept;
             }
             const double exceed = static_cast<double>(u) * static_cast<double>(kept);
-            if (mine && static_cast<double>(with) > exceed && !(static_cast<double>(b.mass) > exceed)) {
-                A.ids[r] = static_cast<uint32_t>(s.list[b.e].place);
+            if (mine && static_cast<double>(with) > exceed && !(static_cast<double>(before) > exceed)) {
+                A.ids[r] = static_cast<uint32_t>(place);
                 if (A.probs) A.probs[r] = static_cast<float>(weight * 0x1p44 / static_cast<double>(kept));
             }
             return;
@@ -584,18 +657,42 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
     if (tid == 0) s.n = 0;
     __syncthreads();
     uint64_t by_min = 0;
-    row.each([&](float x, uint32_t i) {
-        const float t = w.exponent(x);
-        if (!Weights::any(t)) return;
-        if (w.is_heavy(t)) {
-            put(s, x, i);
-            return;
+    const bool bordered = min_p > 0.0f;
+    row.batches([&](const float (&x)[row.kBatch], uint32_t b0) {
+#pragma unroll
+        for (uint32_t q = 0; q < row.kBatch; q += 4) { // four side by side, since each is a chain of slow instructions
+            const float most = fmaxf(fmaxf(x[q], x[q + 1]), fmaxf(x[q + 2], x[q + 3]));
+            if (!Weights::any(w.exponent(most))) continue;
+            float t[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) t[j] = fmaxf(w.exponent(x[q + j]), -64.0f); // (from -inf or NaN too)
+            bool some = most >= w.heavy;
+            if (bordered)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) some |= x[q + j] >= w.border && x[q + j] <= w.passed;
+            if (some)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    if (w.is_heavy(x[q + j]) && Weights::any(t[j])) {
+                        put(s, x[q + j], row.id(b0, q + j));
+                        t[j] = -64.0f;
+                    }
+            uint64_t m[4];
+            uint32_t b[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                m[j] = Weights::light(t[j]); // 0 up to -46
+                b[j] = steps.of(x[q + j]);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[b[j]]), m[j]);
+            if (counted)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) atomicAdd(&s.count[b[j]], Weights::any(t[j]) ? 1u : 0u);
+            if (bordered)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) by_min += x[q + j] > w.passed ? m[j] : 0;
         }
-        const uint32_t b = steps.of(x);
-        const uint64_t m = Weights::light(t);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[b]), m);
-        if (counted) atomicAdd(&s.count[b], 1u);
-        if (t > w.border) by_min += m;
     });
     __syncthreads();
     const auto heavy = [&](float x) {
@@ -612,7 +709,7 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
     } else {
         slow.each([&](float x, uint32_t) {
             const float t = w.exponent(x);
-            if (Weights::any(t) && w.is_heavy(t)) heavy(x);
+            if (Weights::any(t) && w.is_heavy(x)) heavy(x);
         });
     }
     if (min_p > 0.0f && by_min) atomicAdd(reinterpret_cast<unsigned long long *>(&s.kept_by_min), by_min);
@@ -644,7 +741,11 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
         uint64_t m0 = 0;
         uint32_t c0 = 0, step = 0;
         float hi = high, lo = -kInf;
-        if (tid == 0) s.n = 0;
+        if (tid == 0) s.n = s.n2 = 0;
+        if (tid < 64) {
+            s.part_mass[tid] = 0;
+            s.part_count[tid] = 0;
+        }
         if (!spoiled) {
             for (uint32_t i = tid; i < kBins; i += kThreads)
                 if (t.met(s.count[i], s.mass[i]) && (i == 0 || !t.met(s.count[i - 1], s.mass[i - 1]))) s.step = i;
@@ -652,7 +753,9 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
             step = s.step;
             m0 = step ? s.mass[step - 1] : 0;
             c0 = step && counted ? s.count[step - 1] : 0;
-            row.each([&](float x, uint32_t i) {
+            float from, to;
+            steps.reach(step, from, to);
+            row.between(from, to, [&](float x, uint32_t i) {
                 if (steps.of(x) == step && Weights::any(w.exponent(x))) put(s, x, i);
             });
         } else {
@@ -663,6 +766,7 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
         }
         __syncthreads();
         uint32_t n = s.n;
+        const bool in_step = !spoiled && n <= kThreads && n > 32;
         if (n > kThreads) {
             if (!spoiled) { // the step's bounds
                 float a = -kInf, b = kInf;
@@ -705,7 +809,8 @@ template <uint32_t kThreads, bool kWide> __global__ __launch_bounds__(kThreads, 
         }
         if (tid < n) s.list[tid].mass = w.of(logit_of(s.list[tid].place));
         __syncthreads();
-        rank_list<kThreads>(s, t, n, m0, c0);
+        if (in_step) rank_step<kThreads>(s, steps, step, t, n, m0, c0);
+        else rank_list<kThreads>(s, s.list, t, n, m0, c0);
         if (stage < 2) kept = s.cut_mass < kept ? s.cut_mass : kept;
         __syncthreads();
     }
