@@ -6,7 +6,7 @@
 namespace fmx {
 
 uint64_t attention_paged_scratch(const PagedArgs &a, uint32_t type, uint32_t heads) {
-    const Plan p = plan_of(a, type, heads / a.kv_heads);
+    const Plan p = plan_of(a, type, heads / a.kv_heads, kUnbounded); // (a window only lessens the splits)
     return p.splits > 1 ? scratch_of(p.tiles, a.kv_heads, p.splits, p.tile_rows, a.head_dim).total : 0;
 }
 

@@ -16,6 +16,8 @@
 
 #include "paged.hpp"
 
+#include <algorithm>
+
 namespace fmx {
 
 struct AttentionArgs {
@@ -1091,7 +1093,13 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs 
 
 // A split is worth its second launch and its sums' way through memory where
 // the tiles alone leave CUs idle; never into pieces below one unit of keys.
-constexpr uint32_t kFillRows = 2048, kFillTiles = 512; // workgroups that a split aims at
+// Workgroups that a split aims at; an f32 call, whose blocks take 16 times as
+// long, aims at kFillLong where the pieces stay of kLongPiece keys and more, so
+// that tiles of unequal length end together. (us at 512 / 1280: f32, 11 new tokens
+// of 4 sequences over up to 60376 positions, 2 kv heads, 363 / 264; 709 over 1512,
+// 8 heads, whose pieces are shorter, 71 / 77; bf16, a prompt of 4096 tokens, 8
+// heads, 182 / 227, for the sums' way through memory.)
+constexpr uint32_t kFillRows = 2048, kFillTiles = 512, kFillLong = 1280, kLongPiece = 256;
 // Rows of a sequence up to which the 16-row kernel takes a call. 32, 64 and 128
 // rows of 16 sequences over 4096 positions, 8 kv heads of 128, 16-row / 128-row
 // kernel, us: bf16 80 / 57, 126 / 59, 211 / 71; f32 160 / 226, 268 / 407, 485 /
@@ -1111,13 +1119,6 @@ Scratch scratch_of(uint64_t tiles, uint32_t kv_heads, uint32_t splits, uint32_t 
 
 uint64_t tiles_of(const PagedArgs &a, uint32_t group, uint32_t tile_rows) {
     return static_cast<uint64_t>(a.tokens) * group / tile_rows + (a.sequences < a.tokens ? a.sequences : a.tokens);
-}
-
-uint32_t splits_of(const PagedArgs &a, uint64_t tiles, uint32_t unit, uint32_t fill) {
-    const uint64_t blocks = tiles * a.kv_heads;
-    const uint32_t most = div_up(a.max_length, unit);
-    const uint64_t want = (fill + blocks - 1) / blocks;
-    return static_cast<uint32_t>(want < most ? want : most);
 }
 
 template <typename T, int DP> int launch_join(const AttentionArgs &A, uint64_t tiles, uint32_t tile_rows, uint32_t unit,
@@ -1140,21 +1141,29 @@ struct Plan {
     uint32_t tile_rows, unit, splits;
     uint64_t tiles;
 };
-Plan plan_of(const PagedArgs &a, uint32_t type, uint32_t group) {
+Plan plan_of(const PagedArgs &a, uint32_t type, uint32_t group, uint32_t window) {
     Plan p;
     const bool rows = static_cast<uint64_t>(a.max_new) * group <= rows_most(type);
     p.tile_rows = rows ? kRows : kTileRows;
-    p.unit = rows ? (type == FMX_TYPE_F32 ? 16 : 32) * kWaves
-                  : kBlock;
+    p.unit = rows ? (type == FMX_TYPE_F32 ? 16 : 32) * kWaves : kBlock;
     p.tiles = tiles_of(a, group, p.tile_rows);
-    p.splits = splits_of(a, p.tiles, p.unit, rows ? kFillRows : kFillTiles);
+    // keys that a tile's rows see, at most
+    const uint64_t near = static_cast<uint64_t>(window) + p.tile_rows / group + 8;
+    const uint32_t keys = near < a.max_length ? static_cast<uint32_t>(near) : a.max_length;
+    const uint64_t blocks = p.tiles * a.kv_heads;
+    uint64_t want = ((rows ? kFillRows : kFillTiles) + blocks - 1) / blocks;
+    if (!rows && type == FMX_TYPE_F32) {
+        const uint64_t finer = (kFillLong + blocks - 1) / blocks, pieces = keys / kLongPiece;
+        want = std::max(want, std::min(finer, pieces));
+    }
+    p.splits = static_cast<uint32_t>(std::min<uint64_t>(want, div_up(keys, p.unit)));
     return p;
 }
 
 template <typename T, int DP, int DC, int kParts>
 int launch_one(AttentionArgs A, uint8_t *scratch, uint32_t type, hipStream_t s) {
     using Tile = Tile32<T, DP, DC>;
-    const Plan p = plan_of(A.a, type, A.group.d);
+    const Plan p = plan_of(A.a, type, A.group.d, A.window);
     A.splits = p.splits;
     A.stats = reinterpret_cast<float2 *>(scratch);
     A.parts = reinterpret_cast<float *>(scratch + scratch_of(p.tiles, A.a.kv_heads, p.splits, p.tile_rows, A.a.head_dim).stats);
