@@ -6,15 +6,22 @@
 // w = e^((x - M) / T), M the largest logit. Each filter keeps a prefix of that
 // order, so what is kept is the shortest of three prefixes and its mass the
 // least of three masses, and the token is the first whose cumulated mass
-// exceeds uniform x that mass. Nothing is sorted: a place in the order where a
-// count or a mass crosses a target is found by a histogram over equal steps of
-// x, then among the elements of the one step that holds it, every one against
-// every other. A small top-k needs no masses but its own: the k-th largest of
-// the threads' maxima bounds the k-th logit from below, and what lies above
-// that bound is listed in one pass.
+// exceeds uniform x that mass. A place in the order where a count or a mass
+// crosses a target is found by a histogram over equal steps of x, then by the 64
+// parts of the one step that holds it, then among that part's few elements, each
+// against every other. A small top-k needs no masses but its own: the k-th
+// largest of the threads' maxima bounds the k-th logit from below, and what lies
+// above that bound is listed in one pass and ordered.
 //
 // Masses are integers in steps of 2^-44: their sums do not depend on the order
 // of the additions (LDS atomics, whichever wavefront comes first).
+//
+// One workgroup a row, so that a row's passes meet in LDS. One row of 32000 with
+// top-k takes 12 us (5.4 to the maximum, launch included, 5 to list what passes
+// the bound, 2 to order it); 64 rows of 131072 take 20 us with top-k and 52 with
+// top-p alone, 512 rows of 32001 46 us, where a copy would take 6.6, 6.6 and 13:
+// the histogram's pass issues some 17 instructions an element on the one CU that
+// has the row (18 us for 131072), and each pass after the first waits for L2.
 #include "paged.hpp"
 
 namespace fmx {
