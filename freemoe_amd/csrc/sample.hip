@@ -17,8 +17,8 @@
 // of the additions (LDS atomics, whichever wavefront comes first).
 //
 // One workgroup a row, so that a row's passes meet in LDS. One row of 32000 with
-// top-k takes 12 us (5.4 to the maximum, launch included, 5 to list what passes
-// the bound, 2 to order it); 64 rows of 131072 take 20 us with top-k and 52 with
+// top-k takes 13 us (5.4 to the maximum, launch included, 5 to list what passes
+// the bound, 2 to order it); 64 rows of 131072 take 24 us with top-k and 52 with
 // top-p alone, 512 rows of 32001 46 us, where a copy would take 6.6, 6.6 and 13:
 // the histogram's pass issues some 17 instructions an element on the one CU that
 // has the row (18 us for 131072), and each pass after the first waits for L2.

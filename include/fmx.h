@@ -437,8 +437,10 @@ typedef struct fmx_sampling {
  * the first whose cumulated mass exceeds uniform x the mass kept, probs[row]
  * (may be NULL) its share of that mass. Masses are sums of w in 2^-44 steps,
  * the same in whatever order they are added, so a row's token depends on
- * nothing but its inputs. Logits of -inf are never chosen. A row with a NaN or
- * +inf or without a finite logit, a temperature below 0 or a NaN setting gives
+ * nothing but its inputs; w comes from double arithmetic from about 1/8 of the
+ * largest on and next to min_p's border, else from a float's exponential
+ * (within 2^-20 of itself). Logits of -inf are never chosen. A row with a NaN or
+ * +inf or without a finite logit, a temperature below 0, a NaN setting or uniform gives
  * ids[row] = 0xffffffff, probs[row] = 0 and FMX_ERR_INTERNAL from
  * fmx_moe_status. vocab <= 262144. */
 uint64_t fmx_sample_workspace_bytes(uint32_t rows, uint32_t vocab);
