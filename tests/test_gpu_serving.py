@@ -189,6 +189,11 @@ ATTENTION = {
     "prompt_f32_64": (2, 1, 64, F32, F32, 16, [90], [300], {}),
     "split_tiles": (2, 1, 64, BF16, F32, 16, [70], [4100], {}),
     "split_tiles_f32": (1, 1, 32, F32, F32, 16, [70], [2100], dict(window=1999)),
+    "split_tiles_f32_finer": (2, 1, 64, F32, F32, 16, [80, 40], [5200, 300], {}),
+    "split_window_one_token": (8, 2, 64, BF16, F32, 16, [1, 1, 1], [5000, 4097, 3], dict(window=600)),
+    "split_window_tiles": (4, 1, 64, BF16, BF16, 16, [40, 3], [5000, 700], dict(window=700)),
+    "split_window_tiles_f32": (2, 1, 64, F32, F32, 24, [90, 33], [5000, 1600], dict(window=1500)),
+    "split_window_of_one": (4, 1, 64, F16, F32, 16, [1, 2], [900, 901], dict(window=1)),
     "one_row_of_a_tile_more": (1, 1, 128, BF16, BF16, 16, [129, 257], [129, 300], {}),
     "negative_scale": (4, 2, 64, BF16, F32, 16, [1, 70], [90, 70], dict(scale=-0.2)),
     "no_scale": (4, 2, 64, F16, F32, 16, [1, 70], [90, 70], dict(scale=0.0)),
@@ -572,6 +577,47 @@ def test_sample_ties_and_masks(gpu, vocab):
     check_sample(gpu, x, [0.125] * rows, min_p=[1.0] * rows, temperature=[2.0] * rows)
     check_sample(gpu, x, [0.875] * rows, temperature=[math.inf] * rows)
     check_sample(gpu, x, [0.875] * rows, temperature=[1e-45] * rows)
+
+
+@pytest.mark.parametrize("crowd", [31, 33, 64, 65, 400, 511, 513, 1000, 1025, 1500])
+def test_sample_crowds_within_a_step(gpu, crowd):
+    """`crowd` logits that share one of the search's steps, equal or a few last
+    places apart, among 6000 of which the largest is far above: the choice, the
+    end of top-p and of a large top-k fall among them. The largest weighs 1 and
+    the crowd's members 2^-8 of that (their differences are below 2^-20): the
+    distribution's halves and quarters lie inside."""
+    vocab, g = 6000, torch.Generator().manual_seed(crowd)
+    rows = []
+    for spread in (0.0, 2.0 ** -19, 2.0 ** -17):
+        x = torch.full((vocab,), -20.0) - torch.rand(vocab, generator=g) * 5
+        ids = torch.randperm(vocab, generator=g)
+        at = 4.0 - 8 * math.log(2.0)
+        x[ids[:crowd]] = at + torch.randint(0, 8, (crowd,), generator=g) * spread
+        x[ids[crowd]] = 4.0
+        rows.append(x)
+    x = torch.stack(rows).repeat(3, 1)
+    n = x.shape[0]
+    u = [0.97, 0.6, 0.3, 0.9, 0.999, 0.5, 0.85, 0.7, 0.99]
+    check_sample(gpu, x, u)
+    check_sample(gpu, x, u, top_p=[0.9, 0.8, 0.55, 0.99, 0.7, 0.85, 0.6, 0.95, 0.75])
+    check_sample(gpu, x, u, top_k=[300, 257, 999, 20, 30, 1000, 260, 5000, 100])
+    check_sample(gpu, x, u, top_k=[crowd + 1, crowd, crowd // 2 + 1] * 3, top_p=[0.9] * n, min_p=[2.0 ** -8 - 2.0 ** -12] * n)
+
+
+@pytest.mark.parametrize("temperature", [1e-38, 1e-20, 2.0 ** -7, 33.0, 1e10, 3e38])
+def test_sample_at_extreme_temperatures(gpu, temperature):
+    """Weights that are all alike, or but one or two: the filters as ever. Alike
+    weights (the last two) are 1 to the last place, so that their prefixes end
+    where the counts say; u and top_p are odd multiples of 2^-13, never at an
+    element's edge of the 1000 or 5000."""
+    g = torch.Generator().manual_seed(3)
+    for vocab in (1000, 5000):
+        x = torch.randint(-40, 40, (4, vocab), generator=g) * 0.25
+        u = [1.0 / 8192, 4095.0 / 8192, 8191.0 / 8192, 2047.0 / 8192]
+        t = [temperature] * 4
+        check_sample(gpu, x, u, temperature=t)
+        check_sample(gpu, x, u, temperature=t, top_k=[1, 7, 300, 700])
+        check_sample(gpu, x, u, temperature=t, top_p=[4097.0 / 8192] * 4, top_k=[0, 0, 500, 100])
 
 
 def test_sample_refuses_rows_without_a_distribution(gpu):
