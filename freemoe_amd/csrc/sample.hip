@@ -65,9 +65,9 @@ __device__ __forceinline__ double exp2_table(double t, const double *table) {
 
 // A row's weights. Those of about 1 / 8 of the largest and more, and those next
 // to min-p's border, come from double arithmetic ("heavy"); the others, a body
-// that matters by its sum, from v_exp_f32 on an exponent carried to 2^-24 of
-// itself (2^-20 of each weight, 2^-23 of the largest, in either direction, at
-// the very most). Weights below 2^-46 are none.
+// that matters by its sum, from v_exp_f32 on an exponent t that carries two
+// roundings: to (2 |t| ln 2 + 2) 2^-24 of itself, so 2^-24 of the largest weight
+// at the very most and 2^-20 of a weight of 2^-10. Weights below 2^-46 are none.
 struct Weights {
     float M, c_hi, c_lo;          // log 2 units per logit in two floats
     float heavy, border, passed;  // logits: from `heavy` on, and `border` to `passed` (2^-10 around it), in double

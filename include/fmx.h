@@ -439,7 +439,7 @@ typedef struct fmx_sampling {
  * the same in whatever order they are added, so a row's token depends on
  * nothing but its inputs; w comes from double arithmetic from about 1/8 of the
  * largest on and next to min_p's border, else from a float's exponential
- * (within 2^-20 of itself). Logits of -inf are never chosen. A row with a NaN or
+ * (a weight of 2^t to within (2 |t| + 2) 2^-24 of itself). Logits of -inf are never chosen. A row with a NaN or
  * +inf or without a finite logit, a temperature below 0, a NaN setting or uniform gives
  * ids[row] = 0xffffffff, probs[row] = 0 and FMX_ERR_INTERNAL from
  * fmx_moe_status. vocab <= 262144. */

@@ -252,6 +252,28 @@ def test_attention_paged(gpu, name):
     check_attention(P, q, got[:, :H * D].unflatten(1, (H, D)), options, tout, scale)
 
 
+@pytest.mark.parametrize("name", ["decode", "decode_wide_f32", "decode_mqa", "few_tokens", "window", "sinks", "window_f32",
+                                  "more_tokens_than_positions", "many_sequences"])
+@pytest.mark.parametrize("loose", [dict(max_new=400), dict(tokens=700), dict(max_new=90, tokens=100000)])
+def test_attention_paged_with_loose_bounds(gpu, name, loose):
+    """Bounds above what the batch holds choose other kernels and splits, not other
+    results; rows that the arrays do not reach are left alone."""
+    P, q, tout, options = attention_case(name)
+    H, D = q.shape[1:]
+    cache, batch = P.on(gpu)
+    tokens = max(loose.get("tokens", 0), P.tokens)
+    batch = sv.Batch(batch.starts, batch.lengths, batch.table, tokens, max(loose.get("max_new", 0), P.max_new))
+    qd = torch.full((tokens, H, D), float("nan"), dtype=q.dtype, device=gpu)
+    qd[:P.starts[-1]] = q[:P.starts[-1]].to(gpu)
+    out = torch.full((tokens, H, D), 7.0, dtype=tout, device=gpu)
+    ws = sv.attention_workspace(cache, batch, H)
+    on_gpu = {k: to(gpu, v) if torch.is_tensor(v) else v for k, v in options.items()}
+    sv.attention(cache, batch, qd, out, ws, **on_gpu)
+    assert sv.status(ws) == 0
+    assert (out[P.starts[-1]:] == 7.0).all()
+    check_attention(P, q, out[:P.tokens].cpu(), options, tout, 1.0 / math.sqrt(D))
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("counts,window", [([40], 0), ([4], 0), ([40], 12), ([150], 40), ([150], 0)])
 def test_attention_paged_unseen_values_stay_out(gpu, dtype, counts, window):
@@ -515,6 +537,23 @@ def f32(x):
     return float(np.float32(x))
 
 
+def light_error(x, temperature, chosen, p):
+    """Relative error of the mass kept, beyond its steps of 2^-44 of the largest
+    weight. Weights from 1/8 on come from double arithmetic; a smaller one, w = 2^t,
+    from a float t that carries two roundings of 2^-24 of itself (the difference of
+    logits, the product) and an exponential good to a unit in the last place: w
+    times (2 |t| ln 2 + 2) 2^-24. These add up over the light weights at worst (1/7:
+    the border is itself a float), against the mass kept, which is the chosen one's
+    weight over its probability."""
+    if temperature == 0.0:
+        return 0.0
+    x = x.double()
+    t = torch.where(x == -math.inf, -math.inf, (x - x.max()) / f32(temperature)) / math.log(2.0)
+    w = torch.exp2(t)
+    light = (w < 1 / 7) & (t > -47)
+    return float((w[light] * (2 * t[light].abs() * math.log(2.0) + 2)).sum()) * U * p / float(w[chosen])
+
+
 def check_sample(gpu, x, uniform, stride=None, **settings):
     rows, vocab = x.shape
     xd = torch.full((rows, stride or vocab), 1e30, device=gpu)
@@ -529,8 +568,8 @@ def check_sample(gpu, x, uniform, stride=None, **settings):
     for r in range(rows):
         want, p = ref.sample(x[r], f32(uniform[r]), **{k: (f32(v[r]) if k != "top_k" else v[r]) for k, v in settings.items()})
         assert ids[r] == want, (r, {k: v[r] for k, v in settings.items()})
-        # a float's rounding, and masses in steps of 2^-44 of the largest
-        assert abs(probs[r] - p) <= p * U + vocab * 2.0 ** -44, r
+        assert abs(probs[r] - p) <= p * (U + light_error(x[r], settings.get("temperature", [1.0] * rows)[r], want, p)) \
+            + vocab * 2.0 ** -44, r
 
 
 @pytest.mark.parametrize("vocab", [1, 2, 63, 1000, 8192, 8193, 32000, 32769, 131072, 262144])
@@ -602,6 +641,20 @@ def test_sample_crowds_within_a_step(gpu, crowd):
     check_sample(gpu, x, u, top_p=[0.9, 0.8, 0.55, 0.99, 0.7, 0.85, 0.6, 0.95, 0.75])
     check_sample(gpu, x, u, top_k=[300, 257, 999, 20, 30, 1000, 260, 5000, 100])
     check_sample(gpu, x, u, top_k=[crowd + 1, crowd, crowd // 2 + 1] * 3, top_p=[0.9] * n, min_p=[2.0 ** -8 - 2.0 ** -12] * n)
+
+
+@pytest.mark.parametrize("vocab", [1, 700, 1500, 3000, 9001])
+def test_sample_many_rows(gpu, vocab):
+    """Enough rows for two smaller workgroups a CU: every setting at once, and rows
+    of few values, whose crowds pass what such a workgroup lists."""
+    rows, g = 520, torch.Generator().manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=g) * 2
+    x[::5] = torch.randint(0, 3, (len(range(0, rows, 5)), vocab), generator=g).float()
+    pick = lambda *values: [values[int(i)] for i in torch.randint(0, len(values), (rows,), generator=g)]
+    u = torch.rand(rows, generator=g).tolist()
+    check_sample(gpu, x, u, stride=vocab + 1)
+    check_sample(gpu, x, u, temperature=pick(0.0, 0.5, 0.9, 1.7), top_k=pick(0, 1, 40, 256, 257, 2000),
+                 top_p=pick(1.0, 0.9, 0.5), min_p=pick(0.0, 0.05))
 
 
 @pytest.mark.parametrize("temperature", [1e-38, 1e-20, 2.0 ** -7, 33.0, 1e10, 3e38])
