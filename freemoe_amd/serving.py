@@ -30,7 +30,8 @@ class Cache:
     @classmethod
     def of(cls, k: torch.Tensor, v: torch.Tensor) -> "Cache":
         """On existing pools, [page, place, kv head, element] with any strides the library takes."""
-        if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.dim() != 4 or k.stride(3) != 1:
+        if (k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device
+                or k.dim() != 4 or k.stride(3) != 1):
             raise ValueError("k and v: alike, [page, place, kv head, element], elements next to each other")
         self = cls.__new__(cls)
         self.k, self.v = k, v
@@ -52,11 +53,12 @@ class Batch:
 
     def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, tokens: int, max_new: int):
         for t in (starts, lengths, table):
-            if t.dtype != torch.int32 or not t.is_contiguous():
-                raise ValueError("starts, lengths and table: contiguous int32")
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != starts.device:
+                raise ValueError("starts, lengths and table: contiguous int32 on one device")
         if starts.numel() != lengths.numel() + 1 or table.shape[0] != lengths.numel():
             raise ValueError("starts: one more than lengths; table: a row per sequence")
         self.starts, self.lengths, self.table, self.tokens = starts, lengths, table, tokens
+        self.device = starts.device
         self.desc = fmx.PagedBatch(lengths.numel(), tokens, max_new, table.shape[1], starts.data_ptr(),
                                    lengths.data_ptr(), table.data_ptr())
 
@@ -76,7 +78,7 @@ class Rope:
         return fmx.Rope(self.layout, self.dims, self.inv_freq.data_ptr(), self.magnitude, positions)
 
 
-def _rows(t: torch.Tensor, tokens: int, heads: int, head_dim: int, dtype=None) -> int:
+def _rows(t: torch.Tensor, device, tokens: int, heads: int, head_dim: int, dtype=None) -> int:
     """Row stride of [tokens, heads, head_dim] (the heads of a row next to each other)."""
     n, h, d = t.shape
     s0, s1, s2 = t.stride()
@@ -84,16 +86,30 @@ def _rows(t: torch.Tensor, tokens: int, heads: int, head_dim: int, dtype=None) -
         raise ValueError("rows: [tokens, heads, head_dim], a row's heads next to each other")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"rows of {dtype}, not {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"rows on {device}, not {t.device}")
     return s0 if n > 1 else max(s0, h * d)
 
 
-def _entries(t: torch.Tensor | None, count: int, dtype):
+def _entries(t: torch.Tensor | None, device, count: int, dtype):
     """A device array of `count` entries, or NULL."""
     if t is None:
         return None
     if t.dtype != dtype or t.numel() < count or not t.is_contiguous():
         raise ValueError(f"an array of {count} entries of {dtype}, next to each other")
+    if t.device != device:
+        raise ValueError(f"an array on {device}, not {t.device}")
     return t.data_ptr()
+
+
+def _stream(device, stream, *others):
+    """The stream's handle; its GPU, which is the current one, must hold the tensors."""
+    for other in others:
+        if other != device:
+            raise ValueError(f"tensors on {device} and on {other}")
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {device}, which is not the current GPU")
+    return fmx.stream_handle(stream)
 
 
 def workspace(bytes_: int = 256, device="cuda") -> torch.Tensor:
@@ -107,11 +123,12 @@ def status(ws: torch.Tensor, stream=None) -> int:
 
 def rope_append(cache: Cache, batch: Batch, rope: Rope, q, k, v, q_out, ws, positions=None, stream=None):
     n, heads, kv_heads, d, dtype = batch.tokens, q.shape[1], cache.desc.kv_heads, cache.desc.head_dim, q.dtype
+    dev = cache.k.device
     fmx.call("fmx_rope_append", ctypes.byref(cache.desc), ctypes.byref(batch.desc),
-             ctypes.byref(rope.desc(_entries(positions, n, torch.int32))), heads, TYPE_IDS[dtype], q.data_ptr(),
-             _rows(q, n, heads, d), k.data_ptr(), _rows(k, n, kv_heads, d, dtype), v.data_ptr(),
-             _rows(v, n, kv_heads, d, dtype), q_out.data_ptr(), _rows(q_out, n, heads, d, cache.k.dtype), ws.data_ptr(),
-             ws.numel(), fmx.stream_handle(stream))
+             ctypes.byref(rope.desc(_entries(positions, dev, n, torch.int32))), heads, TYPE_IDS[dtype], q.data_ptr(),
+             _rows(q, dev, n, heads, d), k.data_ptr(), _rows(k, dev, n, kv_heads, d, dtype), v.data_ptr(),
+             _rows(v, dev, n, kv_heads, d, dtype), q_out.data_ptr(), _rows(q_out, dev, n, heads, d, cache.k.dtype),
+             _entries(ws, dev, 0, torch.uint8), ws.numel(), _stream(dev, stream, batch.device, rope.inv_freq.device))
     return q_out
 
 
@@ -123,12 +140,13 @@ def attention_workspace(cache: Cache, batch: Batch, heads: int) -> torch.Tensor:
 
 
 def attention(cache: Cache, batch: Batch, q, out, ws, scale=None, softcap=0.0, window=0, sinks=None, stream=None):
-    n, heads, d = batch.tokens, q.shape[1], cache.desc.head_dim
+    n, heads, d, dev = batch.tokens, q.shape[1], cache.desc.head_dim, cache.k.device
     options = fmx.AttentionOptions(1.0 / math.sqrt(d) if scale is None else scale, softcap, window,
-                                   _entries(sinks, heads, torch.float32))
+                                   _entries(sinks, dev, heads, torch.float32))
     fmx.call("fmx_attention_paged", ctypes.byref(cache.desc), ctypes.byref(batch.desc), ctypes.byref(options), heads,
-             q.data_ptr(), _rows(q, n, heads, d, cache.k.dtype), TYPE_IDS[out.dtype], out.data_ptr(),
-             _rows(out, n, heads, d), ws.data_ptr(), ws.numel(), fmx.stream_handle(stream))
+             q.data_ptr(), _rows(q, dev, n, heads, d, cache.k.dtype), TYPE_IDS[out.dtype], out.data_ptr(),
+             _rows(out, dev, n, heads, d), _entries(ws, dev, 0, torch.uint8), ws.numel(),
+             _stream(dev, stream, batch.device))
     return out
 
 
@@ -141,10 +159,10 @@ def sample(logits, uniform, ws=None, temperature=None, top_k=None, top_p=None, m
     ids = torch.empty(rows, dtype=torch.int32, device=logits.device) if ids is None else ids
     probs = torch.empty(rows, dtype=torch.float32, device=logits.device) if probs is None else probs
     ws = workspace(fmx.lib().fmx_sample_workspace_bytes(rows, vocab), logits.device) if ws is None else ws
-    f32 = torch.float32
-    settings = fmx.Sampling(_entries(temperature, rows, f32), _entries(top_k, rows, torch.int32),
-                            _entries(top_p, rows, f32), _entries(min_p, rows, f32))
+    dev, f32, i32 = logits.device, torch.float32, torch.int32
+    settings = fmx.Sampling(_entries(temperature, dev, rows, f32), _entries(top_k, dev, rows, i32),
+                            _entries(top_p, dev, rows, f32), _entries(min_p, dev, rows, f32))
     fmx.call("fmx_sample", logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-             ctypes.byref(settings), _entries(uniform, rows, f32), _entries(ids, rows, torch.int32),
-             _entries(probs, rows, f32), ws.data_ptr(), ws.numel(), fmx.stream_handle(stream))
+             ctypes.byref(settings), _entries(uniform, dev, rows, f32), _entries(ids, dev, rows, i32),
+             _entries(probs, dev, rows, f32), _entries(ws, dev, 0, torch.uint8), ws.numel(), _stream(dev, stream))
     return ids, probs

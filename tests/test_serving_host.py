@@ -145,6 +145,33 @@ def test_tensors_that_do_not_fit_are_refused():
             sv.sample(logits, uniform, ws, **more)
 
 
+def test_tensors_that_are_not_on_the_gpu_are_refused():
+    """Nothing of what the kernels would read may lie in host memory, or on a GPU
+    that is not the current one (here: a device without memory of its own)."""
+    i32 = torch.int32
+    cache = sv.Cache(2, 16, 2, 64, torch.float32, "cpu")
+    batch = sv.Batch(torch.tensor([0, 2], dtype=i32), torch.tensor([5], dtype=i32), torch.zeros(1, 2, dtype=i32), 2, 2)
+    rope, ws = sv.Rope(64, device="cpu"), sv.workspace(device="cpu")
+    q, k = torch.zeros(2, 4, 64), torch.zeros(2, 2, 64)
+    with pytest.raises(ValueError, match="not the current GPU"):
+        sv.attention(cache, batch, q, torch.zeros_like(q), ws)
+    with pytest.raises(ValueError, match="not the current GPU"):
+        sv.rope_append(cache, batch, rope, q, k, k, torch.zeros_like(q), ws)
+    with pytest.raises(ValueError, match="not the current GPU"):
+        sv.sample(torch.zeros(1, 4), torch.zeros(1), ws)
+    elsewhere = torch.zeros(2, 4, 64, device="meta")
+    with pytest.raises(ValueError, match="not meta"):
+        sv.attention(cache, batch, q, elsewhere, ws)
+    with pytest.raises(ValueError, match="not meta"):
+        sv.rope_append(cache, batch, rope, q, k, k, q, ws, positions=torch.zeros(2, dtype=i32, device="meta"))
+    with pytest.raises(ValueError, match="not meta"):
+        sv.sample(torch.zeros(1, 4), torch.zeros(1, device="meta"), ws)
+    with pytest.raises(ValueError, match="alike"):
+        sv.Cache.of(cache.k, cache.v.to("meta"))
+    with pytest.raises(ValueError, match="one device"):
+        sv.Batch(batch.starts, batch.lengths, batch.table.to("meta"), 2, 2)
+
+
 def frequencies(dims, *scaling):
     inv, magnitude = (ctypes.c_double * (dims // 2))(), ctypes.c_double()
     fmx.call("fmx_rope_frequencies", ctypes.byref(fmx.RopeScaling(*scaling)), dims, inv, ctypes.byref(magnitude))
