@@ -208,7 +208,9 @@ int prepare_paged(const fmx_paged_cache *cache, const fmx_paged_batch *batch, Pa
     a->sequences = batch->sequences;
     a->max_new = batch->max_new < batch->tokens ? batch->max_new : batch->tokens;
     a->table_stride = batch->table_stride;
-    a->max_length = positions < 0x7fffffffu ? static_cast<uint32_t>(positions) : 0x7fffffffu;
+    // (kernels look up to 2^12 positions past the last one, in 31 bits)
+    constexpr uint32_t kMost = 0x7fff0000u;
+    a->max_length = positions < kMost ? static_cast<uint32_t>(positions) : kMost;
     a->starts = batch->starts;
     a->lengths = batch->lengths;
     a->table = batch->table;

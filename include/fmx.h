@@ -323,7 +323,7 @@ typedef struct fmx_paged_cache {
  * table_stride bound them from the host:
  *   starts[sequences] <= tokens; rows behind it are neither read nor written
  *   starts[i + 1] - starts[i] <= max_new
- *   lengths[i] <= table_stride * page_size (itself below 2^31)
+ *   lengths[i] <= table_stride * page_size, and at most 2^31 - 2^16
  * An entry that breaks a bound or a page that is not in the pool is not
  * followed: the kernels set a bit that fmx_moe_status reports as
  * FMX_ERR_INVALID_ARGUMENT, and that sequence's results are not meaningful.

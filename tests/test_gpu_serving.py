@@ -376,6 +376,31 @@ def test_attention_paged_reports_what_it_does_not_follow(gpu):
         assert run(change) == (1, True, True)
 
 
+@pytest.mark.parametrize("count", [1, 40])
+@pytest.mark.parametrize("length,status", [(2 ** 31 - 2 ** 16 + 1, 1), (2 ** 31 - 1, 1)])
+def test_paged_lengths_that_pass_31_bits(gpu, count, length, status):
+    """Lengths near 2^31, which a table of 32768 pages of 65536 would cover: past the
+    last one allowed they are reported and not followed, by the cache write either."""
+    D, ps = 8, 65536
+    pool = torch.zeros(1, ps, 1, D, dtype=F16, device=gpu)
+    cache = sv.Cache.of(pool, torch.zeros_like(pool))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=gpu)
+    table = torch.zeros(2, 32768, dtype=torch.int32, device=gpu)
+    batch = sv.Batch(i32(0, count, count + 1), i32(length, 5), table, count + 1, count)
+    q = torch.ones(count + 1, 1, D, dtype=F16, device=gpu)
+    out = torch.full((count + 1, 1, D), 7.0, dtype=F16, device=gpu)
+    ws = sv.attention_workspace(cache, batch, 1)
+    rope = sv.Rope(D, device=gpu)
+    cache.v[0, :5] = 2.0
+    sv.attention(cache, batch, q, out, ws)
+    assert sv.status(ws) == status
+    assert (out[count] == 2.0).all() and (out[:count] == 7.0).all()
+    cache.k.zero_()
+    sv.rope_append(cache, batch, rope, q, q, q, out, ws)
+    assert sv.status(ws) == status
+    assert (cache.k[0, 4] != 0).any() and (cache.k[0, 5:] == 0).all() and (cache.k[0, :4] == 0).all()
+
+
 @pytest.mark.parametrize("dtype,out", [(BF16, F32), (F16, F16), (F32, F32)])
 def test_attention_paged_long(gpu, dtype, out):
     """Long sequences, whose keys go to hundreds of workgroups, beside short ones,
