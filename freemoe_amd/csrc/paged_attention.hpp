@@ -73,15 +73,20 @@ __device__ __forceinline__ Pieces pieces_of(uint32_t keys, uint32_t splits, uint
     return Pieces{each * unit, each ? (units + each - 1) / each : 0};
 }
 
+// The first position that position p sees (p may lie before the first one, far
+// enough that p - window would pass -2^31).
+__device__ __forceinline__ int32_t first_seen(const AttentionArgs &A, int32_t p) {
+    const int32_t window = static_cast<int32_t>(A.window);
+    return A.window != kUnbounded && p >= window ? p - window + 1 : 0;
+}
+
 // The visible keys of rows r0 .. r1 - 1: [lo, hi).
 __device__ __forceinline__ void visible_keys(const AttentionArgs &A, int32_t before, uint32_t r0, uint32_t r1,
                                              int32_t &lo, int32_t &hi) {
     const int32_t first = before + static_cast<int32_t>(A.group.div(r0));
     hi = before + static_cast<int32_t>(A.group.div(r1 - 1)) + 1;
     hi = hi > 0 ? hi : 0;
-    lo = A.window != kUnbounded && first - static_cast<int32_t>(A.window) + 1 > 0
-             ? first - static_cast<int32_t>(A.window) + 1 : 0;
-    lo &= ~7; // the keys of one load instruction share a page where its size allows
+    lo = first_seen(A, first) & ~7; // the keys of one load instruction share a page where its size allows
 }
 
 // Workgroup -> job: splits slowest (so that a tile's workgroups are spread over
@@ -487,11 +492,9 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
     const int32_t p_last = job.before + static_cast<int32_t>(A.group.div(r1 - 1));
     const uint32_t row = r0 + c < r1 ? r0 + c : r1 - 1, token = A.group.div(row), head = kvh * G + row - token * G;
     const int32_t p = job.before + static_cast<int32_t>(token);
-    const bool bounded = A.window != kUnbounded;
-    const int32_t window = static_cast<int32_t>(A.window);
-    const int32_t from = bounded ? p - window + 1 : 0; // first position row c sees
+    const int32_t from = first_seen(A, p);
     // every row of the tile sees these
-    const int32_t all_lo = bounded ? p_last - window + 1 : 0, all_hi = p_first + 1;
+    const int32_t all_lo = first_seen(A, p_last), all_hi = p_first + 1;
 
     Tile tile;
     tile.load_q(A.q + (job.start + token) * A.q_bytes + static_cast<uint64_t>(head) * D * sizeof(T), g, D, A.negate);
@@ -848,14 +851,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attention_tiles_k
     const int32_t p = job.before + static_cast<int32_t>(token);
     const int32_t p_first = job.before + static_cast<int32_t>(A.group.div(active ? w0 : job.r0));
     const int32_t p_last = job.before + static_cast<int32_t>(A.group.div(active ? w1 - 1 : job.r0));
-    const bool bounded = A.window != kUnbounded;
-    const int32_t window = static_cast<int32_t>(A.window);
-    const int32_t from = bounded ? p - window + 1 : 0;
+    const int32_t from = first_seen(A, p);
     // what every row of the workgroup sees, what every row of the wavefront, and
     // where the last of these ends
     const int32_t tile_hi = job.before + static_cast<int32_t>(A.group.div(job.r0)) + 1;
-    const int32_t tile_lo = bounded ? job.before + static_cast<int32_t>(A.group.div(job.r1 - 1)) - window + 1 : 0;
-    const int32_t all_lo = bounded ? p_last - window + 1 : 0, all_hi = p_first + 1;
+    const int32_t tile_lo = first_seen(A, job.before + static_cast<int32_t>(A.group.div(job.r1 - 1)));
+    const int32_t all_lo = first_seen(A, p_last), all_hi = p_first + 1;
     const int32_t any_hi = active ? p_last + 1 : 0;
 
     Tile tile;

@@ -176,6 +176,10 @@ ATTENTION = {
     "peaked": (4, 2, 128, BF16, F32, 16, [5, 70], [300, 70], dict(peak=6.0)),
     "peaked_f16": (4, 2, 128, F16, F32, 16, [5, 70], [300, 70], dict(peak=6.0)),
     "more_tokens_than_positions": (2, 1, 64, BF16, F32, 16, [5, 3], [2, 0], {}),
+    # windows that p - window would carry past -2^31, where a tile begins before the first position
+    "more_tokens_widest_window": (2, 1, 64, BF16, F32, 16, [5, 3, 1], [2, 0, 1], dict(window=2 ** 31 - 1)),
+    "more_tokens_widest_window_tiles": (2, 1, 64, BF16, BF16, 16, [70, 90], [30, 80], dict(window=2 ** 31 - 1)),
+    "more_tokens_window": (2, 1, 64, F32, F32, 16, [70, 9], [30, 4], dict(window=3)),
     "softcap_wide": (4, 2, 64, F32, F32, 16, [3, 80], [90, 130], dict(softcap=50.0)),
     # pages that split a load's rows, and every width the prompt kernels compute at
     "prompt_pages_of_1": (4, 2, 128, BF16, BF16, 1, [70, 40], [130, 41], {}),
