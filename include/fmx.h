@@ -409,9 +409,10 @@ typedef struct fmx_attention_options {
  * included; of those it does see, a score of NaN or +inf makes its row NaN (one
  * of -inf has no weight, and where all have none and there is no sink the row is
  * NaN), and an element of a value that element of its row not finite. Scores and softmax statistics are
- * f32. An f32 result carries f32 accuracy whatever the cache's
- * type; for a 16-bit one the weights are rounded to 16 bits before they meet
- * the values. max_new chooses the kernel: state it as it is. */
+ * f32. An f32 result carries f32 accuracy whatever the cache's type, and a
+ * 16-bit one is that rounded once where max_new x heads / kv_heads is at most
+ * 16; where it is more, a 16-bit result's weights are rounded to 16 bits before
+ * they meet the values. max_new chooses the kernel: state it as it is. */
 uint64_t fmx_attention_paged_workspace_bytes(const fmx_paged_cache *cache, const fmx_paged_batch *batch,
                                              uint32_t heads);
 int fmx_attention_paged(const fmx_paged_cache *cache, const fmx_paged_batch *batch,

@@ -1,0 +1,41 @@
+"""What the serving operators promise beside their values, on an MI355X: how far
+a 16-bit result may lie from the exact one, what may not change a token's bits,
+which entries of a page table are read, on which stream a call's own tensors are
+made."""
+import math
+
+import pytest
+import torch
+
+import serving_ref as ref
+from freemoe_amd import fmx
+from freemoe_amd import serving as sv
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,counts,lengths", [
+    (8, 2, 128, [1, 1, 1], [5000, 300, 2]), (4, 4, 64, [1, 3, 16], [70, 900, 40]), (16, 1, 80, [1, 1], [1300, 64]),
+    (2, 1, 256, [2, 8], [500, 8])])
+def test_few_rows_are_rounded_once(gpu, dtype, heads, kv_heads, dim, counts, lengths):
+    """Up to 16 rows of a sequence in 16 bits: the sums are those of an f32 result,
+    and the one rounding is the output's. The bound is the f32 one (a score's D + 8
+    roundings twice, n sums, some 64 for exponentials, scaling and the weights' last
+    part) with half a step of the output; a weight in 16 bits alone would add half a
+    step of sum_j p_j |v_j|."""
+    P = ref.Paged(counts, lengths, kv_heads, dim, 16, dtype, 71)
+    q = torch.randn(P.tokens, heads, dim, generator=P.g).to(dtype)
+    cache, batch = P.on(gpu)
+    out = torch.zeros(P.tokens, heads, dim, dtype=dtype, device=gpu)
+    ws = sv.attention_workspace(cache, batch, heads)
+    sv.attention(cache, batch, q.to(gpu), out, ws)
+    assert sv.status(ws) == 0
+    got = out.cpu().double()
+    for i, (rows, want, spread, size) in enumerate(ref.attention(P, q, 1.0 / math.sqrt(dim))):
+        error = (2 * U * (dim + 8) * size + U * (lengths[i] + 64)) * spread
+        off = (got[rows] - want).abs() - error - ref.half_step(dtype, want.abs() + error)
+        assert (off <= 0).all(), f"sequence {i}: {off.max()} beyond the bound, {int((off > 0).sum())} of {off.numel()}"
