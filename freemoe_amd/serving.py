@@ -9,6 +9,7 @@ what those hold at each replay.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -113,6 +114,7 @@ def _stream(device, stream, *others):
 
 
 def workspace(bytes_: int = 256, device="cuda") -> torch.Tensor:
+    """Zeroed on the current stream, for which a call on another stream has to wait."""
     return torch.zeros(bytes_, dtype=torch.uint8, device=device)
 
 
@@ -150,19 +152,34 @@ def attention(cache: Cache, batch: Batch, q, out, ws, scale=None, softcap=0.0, w
     return out
 
 
+class Sampled(tuple):
+    """(ids, probs), with the workspace whose error word reports the rows without a distribution."""
+
+    def __new__(cls, ids, probs, ws):
+        self = super().__new__(cls, (ids, probs))
+        self.ids, self.probs, self.ws = ids, probs, ws
+        return self
+
+
 def sample(logits, uniform, ws=None, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, probs=None,
            stream=None):
-    """Token ids (int32) and their probabilities, one per row of logits."""
+    """Token ids (int32) and their probabilities, one per row of logits. A row
+    without a distribution has id -1 and probability 0, and is reported by
+    status(ws), of the result's own `ws` where none is given. What is not given is
+    made on the call's stream, and belongs to it as any tensor of torch does."""
     rows, vocab = logits.shape
     if logits.dtype != torch.float32 or (vocab > 1 and logits.stride(1) != 1):
         raise ValueError("logits: float32 rows")
-    ids = torch.empty(rows, dtype=torch.int32, device=logits.device) if ids is None else ids
-    probs = torch.empty(rows, dtype=torch.float32, device=logits.device) if probs is None else probs
-    ws = workspace(fmx.lib().fmx_sample_workspace_bytes(rows, vocab), logits.device) if ws is None else ws
+    # (another stream's blocks may still be written there, and a workspace that ends
+    # with this call may be handed out again while the kernel runs)
+    with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+        ids = torch.empty(rows, dtype=torch.int32, device=logits.device) if ids is None else ids
+        probs = torch.empty(rows, dtype=torch.float32, device=logits.device) if probs is None else probs
+        ws = workspace(fmx.lib().fmx_sample_workspace_bytes(rows, vocab), logits.device) if ws is None else ws
     dev, f32, i32 = logits.device, torch.float32, torch.int32
     settings = fmx.Sampling(_entries(temperature, dev, rows, f32), _entries(top_k, dev, rows, i32),
                             _entries(top_p, dev, rows, f32), _entries(min_p, dev, rows, f32))
     fmx.call("fmx_sample", logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
              ctypes.byref(settings), _entries(uniform, dev, rows, f32), _entries(ids, dev, rows, i32),
              _entries(probs, dev, rows, f32), _entries(ws, dev, 0, torch.uint8), ws.numel(), _stream(dev, stream))
-    return ids, probs
+    return Sampled(ids, probs, ws)

@@ -39,3 +39,27 @@ def test_few_rows_are_rounded_once(gpu, dtype, heads, kv_heads, dim, counts, len
         error = (2 * U * (dim + 8) * size + U * (lengths[i] + 64)) * spread
         off = (got[rows] - want).abs() - error - ref.half_step(dtype, want.abs() + error)
         assert (off <= 0).all(), f"sequence {i}: {off.max()} beyond the bound, {int((off > 0).sum())} of {off.numel()}"
+
+
+def test_sample_on_another_stream_with_its_own_tensors(gpu):
+    """The current stream's memory is handed out again while its work still writes
+    there: what a call on another stream makes for itself is not of that memory."""
+    rows, vocab = 64, 20000
+    g = torch.Generator(device=gpu).manual_seed(91)
+    x, u = torch.randn(rows, vocab, generator=g, device=gpu), torch.rand(rows, generator=g, device=gpu)
+    x[5, 7] = math.nan
+    want = sv.sample(x, u)
+    assert sv.status(want.ws) == 4 and want.ids[5] == -1 and want.probs[5] == 0
+    side, a = torch.cuda.Stream(), torch.randn(4096, 4096, device=gpu)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        held = [torch.empty(rows, dtype=torch.int32, device=gpu) for _ in range(40)]
+        for _ in range(8):
+            a = a @ a * 1e-3  # some milliseconds
+        for t in held:
+            t.fill_(7)
+        del held, t
+        got = sv.sample(x, u, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(got.ids, want.ids) and torch.equal(got.probs, want.probs)
+        assert sv.status(got.ws, side) == 4 and sv.status(got.ws, side) == 0
