@@ -103,8 +103,15 @@ def _entries(t: torch.Tensor | None, device, count: int, dtype):
     return t.data_ptr()
 
 
+def _same_gpu(device, stream):
+    """A stream of another GPU would run the kernels there. (What only has a handle is taken, as by stream_handle.)"""
+    if getattr(stream, "device", device) != device:
+        raise ValueError(f"a stream of {stream.device} for tensors on {device}")
+
+
 def _stream(device, stream, *others):
     """The stream's handle; its GPU, which is the current one, must hold the tensors."""
+    _same_gpu(device, stream)
     for other in others:
         if other != device:
             raise ValueError(f"tensors on {device} and on {other}")
@@ -170,6 +177,7 @@ def sample(logits, uniform, ws=None, temperature=None, top_k=None, top_p=None, m
     rows, vocab = logits.shape
     if logits.dtype != torch.float32 or (vocab > 1 and logits.stride(1) != 1):
         raise ValueError("logits: float32 rows")
+    _same_gpu(logits.device, stream)
     # (another stream's blocks may still be written there, and a workspace that ends
     # with this call may be handed out again while the kernel runs)
     with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):

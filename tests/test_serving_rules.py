@@ -40,3 +40,19 @@ def test_sample_makes_its_tensors_on_the_calls_stream(monkeypatch):
         assert ids is got.ids and probs is got.probs and got.ws.dtype == torch.uint8 and got.ws.numel() >= 256
     ws = torch.zeros(256, dtype=torch.uint8)
     assert sv.sample(x, u, ws).ws is ws
+
+
+def test_a_stream_of_another_device_is_refused():
+    i32 = torch.int32
+    cache = sv.Cache(2, 16, 2, 64, torch.float32, "cpu")
+    batch = sv.Batch(torch.tensor([0, 2], dtype=i32), torch.tensor([5], dtype=i32), torch.zeros(1, 2, dtype=i32), 2, 2)
+    rope, ws = sv.Rope(64, device="cpu"), sv.workspace(device="cpu")
+    q, k = torch.zeros(2, 4, 64), torch.zeros(2, 2, 64)
+    other = types.SimpleNamespace(cuda_stream=7, device=torch.device("cuda", 1))
+    with pytest.raises(ValueError, match="a stream of cuda:1"):
+        sv.attention(cache, batch, q, torch.zeros_like(q), ws, stream=other)
+    with pytest.raises(ValueError, match="a stream of cuda:1"):
+        sv.rope_append(cache, batch, rope, q, k, k, torch.zeros_like(q), ws, stream=other)
+    for given in (ws, None):
+        with pytest.raises(ValueError, match="a stream of cuda:1"):
+            sv.sample(torch.zeros(1, 4), torch.zeros(1), given, stream=other)
