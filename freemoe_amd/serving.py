@@ -89,7 +89,7 @@ def _rows(t: torch.Tensor, device, tokens: int, heads: int, head_dim: int, dtype
         raise ValueError(f"rows of {dtype}, not {t.dtype}")
     if t.device != device:
         raise ValueError(f"rows on {device}, not {t.device}")
-    return s0 if n > 1 else max(s0, h * d)
+    return s0 if n > 1 else h * d  # (one row's stride is never used, and torch may give it any)
 
 
 def _entries(t: torch.Tensor | None, device, count: int, dtype):

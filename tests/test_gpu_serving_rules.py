@@ -63,3 +63,24 @@ def test_sample_on_another_stream_with_its_own_tensors(gpu):
         torch.cuda.synchronize()
         assert torch.equal(got.ids, want.ids) and torch.equal(got.probs, want.probs)
         assert sv.status(got.ws, side) == 4 and sv.status(got.ws, side) == 0
+
+
+def test_one_row_of_any_stride(gpu):
+    """A tensor of one row has no stride to speak of: a slice of a row whose width
+    no 16 bytes divide is taken."""
+    H, G, D = 2, 1, 24
+    P = ref.Paged([1], [30], G, D, 16, F32, 41, spare=0)
+    wide = torch.randn(2, (H + 2 * G) * D + 3, generator=P.g)
+    x = wide.to(gpu)[:, :(H + 2 * G) * D].unflatten(1, (H + 2 * G, D))[:1]
+    cache, batch = P.on(gpu)
+    rope, ws = sv.Rope(D, device=gpu), sv.attention_workspace(cache, batch, H)
+    turned = torch.zeros(2, H * D + 1, device=gpu)[:, :H * D].unflatten(1, (H, D))[:1]
+    sv.rope_append(cache, batch, rope, x[:, :H], x[:, H:H + G], x[:, H + G:], turned, ws)
+    out = torch.zeros(2, H * D + 1, device=gpu)[:, :H * D].unflatten(1, (H, D))[:1]
+    sv.attention(cache, batch, turned, out, ws)
+    assert sv.status(ws) == 0
+    same = torch.zeros(1, H, D, device=gpu)
+    sv.attention(cache, batch, turned.contiguous(), same, ws)
+    assert torch.equal(out, same) and (out != 0).any()
+    want, size = ref.rope(wide[:1, :H * D].unflatten(1, (H, D)), torch.tensor([29]), rope.inv_freq.cpu(), 1.0, D, True)
+    assert ((turned.cpu().double() - want).abs() <= 4 * U * size + U * want.abs()).all()
