@@ -390,28 +390,34 @@ template <int DP> struct Tile16<float, DP> {
 // Scores from q . k, in units of 1 / per_score of log 2: q . k itself, or the
 // capped score. Below 1 / 4, where scores mostly lie, the hyperbolic tangent is
 // its Taylor sum to x^9 (the next term is below 2^-26 of it), a fifth of
-// tanhf's instructions.
+// tanhf's instructions. Which of the two a score takes goes by that score alone,
+// whatever the others of the wavefront are (keys its row does not see among
+// them); their vote only decides whether tanhf has to be computed at all. (A
+// prompt of 4096 in bf16: 170 us without a cap, 223 with scores of a thirtieth of
+// it, 430 with scores about as large as it.)
 template <class Scores> __device__ __forceinline__ void cap_scores(const AttentionArgs &A, Scores &s) {
     constexpr int kN = sizeof(Scores) / sizeof(float);
     if (A.softcap == 0.0f) return;
+    constexpr float kNear = 0.25f;
+    const auto near = [](float x) {
+        const float q = x * x;
+        float t = fma_rn(q, 62.0f / 2835.0f, -17.0f / 315.0f);
+        t = fma_rn(t, q, 2.0f / 15.0f);
+        t = fma_rn(t, q, -1.0f / 3.0f);
+        return fma_rn(t * q, x, x);
+    };
     float most = 0.0f;
 #pragma unroll
     for (int x = 0; x < kN; ++x) {
         s[x] *= A.scale;
         most = fmaxf(most, fabsf(s[x])); // (a NaN is dropped here and kept by either form)
     }
-    if (__any(most > 0.25f)) {
+    if (__any(most > kNear)) {
 #pragma unroll
-        for (int x = 0; x < kN; ++x) s[x] = tanhf(s[x]) * A.softcap;
+        for (int x = 0; x < kN; ++x) s[x] = (fabsf(s[x]) > kNear ? tanhf(s[x]) : near(s[x])) * A.softcap;
     } else {
 #pragma unroll
-        for (int x = 0; x < kN; ++x) {
-            const float q = s[x] * s[x];
-            float t = fma_rn(q, 62.0f / 2835.0f, -17.0f / 315.0f);
-            t = fma_rn(t, q, 2.0f / 15.0f);
-            t = fma_rn(t, q, -1.0f / 3.0f);
-            s[x] = fma_rn(t * q, s[x], s[x]) * A.softcap;
-        }
+        for (int x = 0; x < kN; ++x) s[x] = near(s[x]) * A.softcap;
     }
 }
 

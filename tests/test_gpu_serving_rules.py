@@ -84,3 +84,39 @@ def test_one_row_of_any_stride(gpu):
     assert torch.equal(out, same) and (out != 0).any()
     want, size = ref.rope(wide[:1, :H * D].unflatten(1, (H, D)), torch.tensor([29]), rope.inv_freq.cpu(), 1.0, D, True)
     assert ((turned.cpu().double() - want).abs() <= 4 * U * size + U * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("softcap", [3.0, 50.0])
+@pytest.mark.parametrize("counts", [[4], [40], [150]])
+def test_softcap_of_unseen_keys_stays_out(gpu, dtype, counts, softcap):
+    """Soft-capped scores of keys a token does not see, however large, and of other
+    tokens' queries leave its bits alone: hidden keys, places behind the last one
+    of its page, and the last token's query are made large in turn."""
+    H, G, D, L, n = 4, 2, 64, 165, counts[0]
+    P = ref.Paged(counts, [L], G, D, 16, dtype, 29)
+    for pool, _ in P.pools:
+        pool.nan_to_num_(0.01)
+    # scores of about a twentieth of the cap, none near a quarter of it
+    q = (torch.randn(P.tokens, H, D, generator=P.g) * 0.05 * softcap).to(dtype)
+    at = P.table[0].long()
+
+    def run():
+        cache, batch = P.on(gpu)
+        out = torch.zeros(P.tokens, H, D, device=gpu)
+        ws = sv.attention_workspace(cache, batch, H)
+        sv.attention(cache, batch, q.to(gpu), out, ws, softcap=softcap)
+        assert sv.status(ws) == 0
+        return out.cpu()
+
+    clean = run()
+    keys = P.pools[0][1]
+    keys[at[L // 16], L % 16:] = 40.0  # behind the last position, in its page
+    assert torch.equal(run()[:n], clean[:n])
+    keys[at[(L - 1) // 16], (L - 1) % 16] = 40.0  # the last position: its own token sees it
+    assert torch.equal(run()[:n - 1], clean[:n - 1])
+    j = L - n // 2  # seen from token n - n // 2 on
+    keys[at[j // 16], j % 16] = -40.0
+    assert torch.equal(run()[:n - n // 2], clean[:n - n // 2])
+    q[n - 1] = 40.0
+    assert torch.equal(run()[:n - n // 2], clean[:n - n // 2])
