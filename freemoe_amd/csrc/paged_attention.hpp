@@ -80,13 +80,19 @@ __device__ __forceinline__ int32_t first_seen(const AttentionArgs &A, int32_t p)
     return A.window != kUnbounded && p >= window ? p - window + 1 : 0;
 }
 
-// The visible keys of rows r0 .. r1 - 1: [lo, hi).
+// The visible keys of rows r0 .. r1 - 1: [lo, hi). lo is brought down to a
+// multiple of 8, so that the keys of one load instruction share a page where its
+// size allows, but not out of its page: an earlier one may have been given back.
+// (A page whose size is a multiple of a load's rows, at most 8, starts at one.)
 __device__ __forceinline__ void visible_keys(const AttentionArgs &A, int32_t before, uint32_t r0, uint32_t r1,
                                              int32_t &lo, int32_t &hi) {
     const int32_t first = before + static_cast<int32_t>(A.group.div(r0));
     hi = before + static_cast<int32_t>(A.group.div(r1 - 1)) + 1;
     hi = hi > 0 ? hi : 0;
-    lo = first_seen(A, first) & ~7; // the keys of one load instruction share a page where its size allows
+    const int32_t seen = first_seen(A, first);
+    const int32_t page = static_cast<int32_t>(A.a.page.div(seen) * A.a.page.d); // its first position
+    lo = seen & ~7;
+    lo = lo > page ? lo : page;
 }
 
 // Workgroup -> job: splits slowest (so that a tile's workgroups are spread over

@@ -327,8 +327,9 @@ typedef struct fmx_paged_cache {
  * An entry that breaks a bound or a page that is not in the pool is not
  * followed: the kernels set a bit that fmx_moe_status reports as
  * FMX_ERR_INVALID_ARGUMENT, and that sequence's results are not meaningful.
- * Entries of the table behind a sequence's last page are not read. Sequences
- * may share pages that none of them writes. */
+ * Entries of the table behind a sequence's last page are not read, nor, by an
+ * attention with a window, those of pages that end before the first position a
+ * new token sees. Sequences may share pages that none of them writes. */
 typedef struct fmx_paged_batch {
     uint32_t sequences;
     uint32_t tokens;

@@ -120,3 +120,27 @@ def test_softcap_of_unseen_keys_stays_out(gpu, dtype, counts, softcap):
     assert torch.equal(run()[:n - n // 2], clean[:n - n // 2])
     q[n - 1] = 40.0
     assert torch.equal(run()[:n - n // 2], clean[:n - n // 2])
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(BF16, 128, 12), (F16, 64, 1), (F32, 64, 3), (BF16, 256, 6), (F16, 128, 5),
+                                            (F32, 96, 20), (BF16, 64, 16)])
+@pytest.mark.parametrize("count,window", [(1, 20), (1, 1), (40, 33), (150, 50)])
+def test_pages_before_the_window_are_not_read(gpu, dtype, dim, page, count, window):
+    """A program that slides a window gives back the pages before it: their entries
+    may hold anything, whatever the page size."""
+    H, G, L = 4, 2, 333
+    P = ref.Paged([count, 1], [L, 7], G, dim, page, dtype, 37)
+    q = torch.randn(P.tokens, H, dim, generator=P.g).to(dtype)
+    cache, batch = P.on(gpu)
+    first = L - count - window + 1  # the first position any new token sees
+    gone = first // page
+    assert gone > 0
+    batch.table[0, :gone] = torch.tensor([-1, 10 ** 6] * gone, dtype=torch.int32, device=gpu)[:gone]
+    out = torch.zeros(P.tokens, H, dim, device=gpu)
+    ws = sv.attention_workspace(cache, batch, H)
+    sv.attention(cache, batch, q.to(gpu), out, ws, window=window)
+    assert sv.status(ws) == 0
+    got = out.cpu().double()
+    for i, (rows, want, spread, size) in enumerate(ref.attention(P, q, 1.0 / math.sqrt(dim), window=window)):
+        error = (2 * U * (dim + 8) * size + U * (L + 64)) * spread
+        assert ((got[rows] - want).abs() <= error + ref.half_step(F32, want.abs() + error)).all(), i
