@@ -740,6 +740,9 @@ int fmx_attention_paged(const fmx_paged_cache *cache, const fmx_paged_batch *bat
     if (int rc = prepare_paged(cache, batch, &a)) return rc;
     if (!options || !(std::fabs(options->scale) < 0x1p100) || !(options->softcap >= 0.0) || !(options->softcap < 0x1p100))
         return FMX_ERR_INVALID_ARGUMENT;
+    // the kernels hold the cap and scale / cap in floats
+    if (options->softcap != 0.0 && (options->softcap < 0x1p-126 || std::fabs(options->scale) / options->softcap >= 0x1p127))
+        return FMX_ERR_INVALID_ARGUMENT;
     if (out_type != FMX_TYPE_F32 && out_type != cache->type) return FMX_ERR_UNSUPPORTED_QUANTISATION;
     if (heads == 0 || heads > 65535 || heads % cache->kv_heads) return FMX_ERR_SHAPE_MISMATCH;
     if (a.tokens == 0) return FMX_OK;

@@ -393,8 +393,9 @@ int fmx_rope_append(const fmx_paged_cache *cache, const fmx_paged_batch *batch, 
                     void *workspace, uint64_t workspace_bytes, void *stream);
 
 typedef struct fmx_attention_options {
-    double scale;        /* of q . k; 1 / sqrt(head_dim) as a rule */
-    double softcap;      /* c > 0: scores become c tanh(score / c); 0: as they are */
+    double scale;        /* of q . k; 1 / sqrt(head_dim) as a rule; below 2^100 in size */
+    double softcap;      /* c > 0: scores become c tanh(score / c); 0: as they are. From 2^-126 on,
+                            below 2^100, and scale / c below 2^127 */
     uint32_t window;     /* positions a token sees, its own the last; 0: all before it */
     const float *sinks;  /* device [heads] logits that join each head's softmax without a value, or NULL */
 } fmx_attention_options;

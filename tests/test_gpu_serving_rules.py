@@ -144,3 +144,27 @@ def test_pages_before_the_window_are_not_read(gpu, dtype, dim, page, count, wind
     for i, (rows, want, spread, size) in enumerate(ref.attention(P, q, 1.0 / math.sqrt(dim), window=window)):
         error = (2 * U * (dim + 8) * size + U * (L + 64)) * spread
         assert ((got[rows] - want).abs() <= error + ref.half_step(F32, want.abs() + error)).all(), i
+
+
+@pytest.mark.parametrize("scale,cap", [(0.125, 1e-30), (1e20, 1e-10), (0.0, 2.0 ** -126), (0.125, 2.0 ** 99), (-1e15, 4.0)])
+@pytest.mark.parametrize("dtype,counts", [(F32, [5]), (BF16, [70])])
+def test_extreme_softcaps(gpu, dtype, counts, scale, cap):
+    """The smallest and largest caps a call takes, down to scores that all are 0 or
+    plus and minus the cap (q . k = 0 stays 0 there)."""
+    H, G, D, L = 2, 1, 64, 100
+    P = ref.Paged(counts, [L], G, D, 16, dtype, 43)
+    P.pools[0][1][P.table[0].long()[3], 2] = 0.0  # one key of zeros
+    q = torch.randn(P.tokens, H, D, generator=P.g).to(dtype)
+    cache, batch = P.on(gpu)
+    out = torch.zeros(P.tokens, H, D, device=gpu)
+    ws = sv.attention_workspace(cache, batch, H)
+    sv.attention(cache, batch, q.to(gpu), out, ws, scale=scale, softcap=cap)
+    assert sv.status(ws) == 0
+    got = out.cpu().double()
+    for rows, want, spread, size in ref.attention(P, q, scale, softcap=cap):
+        # a score's error: the roundings of its dot and of the few steps behind it, which
+        # the tangent passes on at most once; of a scale far above the cap the side q . k
+        # lies on is all that counts, and what is left are the cap's own roundings
+        score = (D + 16) * size if abs(scale) <= 1e9 * cap else 8 * cap
+        error = (2 * U * score + U * (L + 64)) * spread
+        assert ((got[rows] - want).abs() <= error + ref.half_step(F32, want.abs() + error)).all()

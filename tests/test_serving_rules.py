@@ -1,5 +1,6 @@
 """What the serving module and calls promise beside their values, on the host."""
 import contextlib
+import ctypes
 import types
 
 import pytest
@@ -56,3 +57,30 @@ def test_a_stream_of_another_device_is_refused():
     for given in (ws, None):
         with pytest.raises(ValueError, match="a stream of cuda:1"):
             sv.sample(torch.zeros(1, 4), torch.zeros(1), given, stream=other)
+
+
+@pytest.fixture
+def buffer():
+    """An aligned host address that no refused call reads."""
+    data = torch.zeros(4096)
+    return data, data.data_ptr() + (-data.data_ptr()) % 256
+
+
+def attention(p, heads=4, tokens=0, max_new=1, options=(0.125, 0.0, 0, None), out_stride=256, **batch):
+    """fmx_attention_paged on descriptors without work unless `tokens` says so."""
+    cache = fmx.PagedCache(fmx.FMX_TYPE_BF16, 2, 64, 16, 8, 2048, 128, 64, p, p)
+    b = dict(sequences=1, tokens=tokens, max_new=max_new, table_stride=4, starts=p, lengths=p, table=p)
+    b.update(batch)
+    return fmx.lib().fmx_attention_paged(ctypes.byref(cache), ctypes.byref(fmx.PagedBatch(*b.values())),
+                                         ctypes.byref(fmx.AttentionOptions(*options)), heads, p, 256, 0, p, out_stride, p,
+                                         1 << 62, None)
+
+
+def test_softcaps_that_a_float_does_not_hold_are_refused(buffer):
+    """Below a float's normal values, or with a scale over it that passes them, the
+    kernels would leave the cap out or turn scores of 0 into NaN."""
+    _, p = buffer
+    for scale, cap in ((0.125, 1e-46), (0.125, 5e-324), (0.0, 1e-50), (0.125, 1e-39), (-1e25, 1e-20), (1e30, 1e-10), (2.0 ** 99, 2.0 ** -28)):
+        assert attention(p, options=(scale, cap, 0, None)) == 1, (scale, cap)
+    for scale, cap in ((0.125, 1e-30), (0.0, 2.0 ** -126), (-1e20, 1e-10), (0.125, 50.0), (1e-300, 2.0 ** 99), (2.0 ** 99, 1.0), (1.0, 0.0)):
+        assert attention(p, options=(scale, cap, 0, None)) == 0, (scale, cap)  # (nothing to do: no launch)
