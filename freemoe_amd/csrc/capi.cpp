@@ -710,6 +710,7 @@ int fmx_rope_append(const fmx_paged_cache *cache, const fmx_paged_batch *batch, 
     if (in_type != FMX_TYPE_F32 && in_type != cache->type) return FMX_ERR_UNSUPPORTED_QUANTISATION;
     if (heads == 0 || heads > 65535 || rope->dims % 2 || rope->dims > cache->head_dim) return FMX_ERR_SHAPE_MISMATCH;
     if (a.tokens == 0) return FMX_OK;
+    if (!launch_fits(a.tokens, kRopeThreads)) return FMX_ERR_SHAPE_MISMATCH;
     if (!q || !k || !v || !q_out || !workspace || workspace_bytes < kStatusBytes || (rope->dims && !rope->inv_freq))
         return FMX_ERR_INVALID_ARGUMENT;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(workspace))
@@ -768,7 +769,8 @@ int fmx_sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t
                void *stream) {
     if (int rc = fault_gate()) return rc;
     if (!sampling) return FMX_ERR_INVALID_ARGUMENT;
-    if (vocab == 0 || vocab > kSampleMaxVocab || row_stride < vocab || rows > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
+    if (vocab == 0 || vocab > kSampleMaxVocab || row_stride < vocab || !launch_fits(rows, kSampleThreads))
+        return FMX_ERR_SHAPE_MISMATCH;
     if (rows == 0) return FMX_OK;
     if (!logits || !uniform || !ids || !workspace || !aligned16(workspace)) return FMX_ERR_INVALID_ARGUMENT;
     if (reinterpret_cast<uintptr_t>(logits) & 3u) return FMX_ERR_INVALID_ARGUMENT;

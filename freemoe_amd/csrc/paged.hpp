@@ -28,6 +28,11 @@ struct PagedArgs {
     const uint32_t *starts, *lengths, *table;
 };
 
+// A launch takes fewer than 2^32 threads in a dimension.
+constexpr bool launch_fits(uint64_t workgroups, uint32_t threads) { return workgroups <= 0xffffffffu / threads; }
+constexpr uint32_t kRopeThreads = 256;
+constexpr uint32_t kSampleThreads = 512; // of a workgroup, where rows are many
+
 inline uint32_t element_bytes(uint32_t type) {
     return type == FMX_TYPE_F32 ? 4 : type == FMX_TYPE_F16 || type == FMX_TYPE_BF16 ? 2 : 0;
 }

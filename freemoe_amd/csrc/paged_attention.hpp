@@ -1162,8 +1162,9 @@ template <typename T, int DP> int launch_join(const AttentionArgs &A, uint64_t t
     if (A.splits <= 1) return FMX_OK;
     constexpr uint32_t kSlots = kThreads / (DP / 4);
     const bool many = A.splits > 8;
+    // (a call is split while its tiles times kv heads are below the workgroups
+    // aimed at: a small grid)
     const uint64_t blocks = tiles * A.a.kv_heads * (tile_rows / (many ? 1 : kSlots));
-    if (blocks > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
     const auto kernel = many ? attention_join_kernel<DP, kSlots> : attention_join_kernel<DP, 1>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, s, A, tile_rows, unit,
                        Element<T>::kLift);
@@ -1204,7 +1205,7 @@ int launch_one(AttentionArgs A, uint8_t *scratch, uint32_t type, hipStream_t s) 
     A.stats = reinterpret_cast<float2 *>(scratch);
     A.parts = reinterpret_cast<float *>(scratch + scratch_of(p.tiles, A.a.kv_heads, p.splits, p.tile_rows, A.a.head_dim).stats);
     const uint64_t blocks = p.tiles * A.a.kv_heads * p.splits;
-    if (blocks > 0x7fffffffu) return FMX_ERR_SHAPE_MISMATCH;
+    if (!launch_fits(blocks, kThreads)) return FMX_ERR_SHAPE_MISMATCH;
     const bool rows = p.tile_rows == kRows;
     const size_t lds = rows ? kWaves * kRows * (DP + 4) * sizeof(float)
                             : kBlock * (Tile::kRing * 2 * DP * sizeof(T) + Tile::kGranules);

@@ -20,7 +20,7 @@ namespace fmx {
 
 namespace {
 
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kThreads = kRopeThreads;
 constexpr uint32_t kMaxPairs = 128;
 
 struct RopeArgs {

@@ -837,10 +837,11 @@ int sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t voc
     const SampleArgs A{logits, row_stride, vocab, p, uniform, ids, probs, status};
     // two workgroups of 512 a CU take turns at what few of their threads do;
     // where rows leave CUs to themselves, one of 1024
-    const uint32_t threads = rows >= 512 ? 512 : 1024;
+    const uint32_t threads = rows >= 512 ? kSampleThreads : 1024;
     const bool wide = vocab > 4 * threads;
-    const auto kernel = threads == 512 ? (wide ? sample_kernel<512, true> : sample_kernel<512, false>)
-                                       : (wide ? sample_kernel<1024, true> : sample_kernel<1024, false>);
+    constexpr uint32_t kMany = kSampleThreads;
+    const auto kernel = threads == kMany ? (wide ? sample_kernel<kMany, true> : sample_kernel<kMany, false>)
+                                         : (wide ? sample_kernel<1024, true> : sample_kernel<1024, false>);
     hipLaunchKernelGGL(kernel, dim3(rows), dim3(threads), 0, s, A);
     FMX_LAUNCH_CHECK();
     return FMX_OK;

@@ -384,7 +384,7 @@ typedef struct fmx_rope {
  * of the cache's type, and the cache's. Angles are formed and reduced in
  * double, pairs turned in f32, each result rounded once; elements from dims on
  * are copied. q_out may be q where types and strides agree. Strides are
- * multiples of 16 bytes, pointers 16-byte aligned. workspace: >= 256 bytes,
+ * multiples of 16 bytes, pointers 16-byte aligned, tokens below 2^24. workspace: >= 256 bytes,
  * the error word (also set, and the token skipped, where a sequence has more
  * new tokens than positions). */
 int fmx_rope_append(const fmx_paged_cache *cache, const fmx_paged_batch *batch, const fmx_rope *rope,
@@ -414,7 +414,10 @@ typedef struct fmx_attention_options {
  * f32. An f32 result carries f32 accuracy whatever the cache's type, and a
  * 16-bit one is that rounded once where max_new x heads / kv_heads is at most
  * 16; where it is more, a 16-bit result's weights are rounded to 16 bits before
- * they meet the values. max_new chooses the kernel: state it as it is. */
+ * they meet the values. max_new chooses the kernel: state it as it is. Refused as
+ * SHAPE_MISMATCH where the call would take 2^24 workgroups: kv_heads times
+ * sequences + tokens x heads / kv_heads / 16 (/ 128 above 16 rows a sequence; 64 in
+ * f32). */
 uint64_t fmx_attention_paged_workspace_bytes(const fmx_paged_cache *cache, const fmx_paged_batch *batch,
                                              uint32_t heads);
 int fmx_attention_paged(const fmx_paged_cache *cache, const fmx_paged_batch *batch,
@@ -445,7 +448,7 @@ typedef struct fmx_sampling {
  * (a weight of 2^t to within (2 |t| + 2) 2^-24 of itself). Logits of -inf are never chosen. A row with a NaN or
  * +inf or without a finite logit, a temperature below 0, a NaN setting or uniform gives
  * ids[row] = 0xffffffff, probs[row] = 0 and FMX_ERR_INTERNAL from
- * fmx_moe_status. vocab <= 262144. */
+ * fmx_moe_status. vocab <= 262144, rows below 2^23. */
 uint64_t fmx_sample_workspace_bytes(uint32_t rows, uint32_t vocab);
 int fmx_sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
                const fmx_sampling *sampling, const float *uniform, uint32_t *ids, float *probs,

@@ -84,3 +84,23 @@ def test_softcaps_that_a_float_does_not_hold_are_refused(buffer):
         assert attention(p, options=(scale, cap, 0, None)) == 1, (scale, cap)
     for scale, cap in ((0.125, 1e-30), (0.0, 2.0 ** -126), (-1e20, 1e-10), (0.125, 50.0), (1e-300, 2.0 ** 99), (2.0 ** 99, 1.0), (1.0, 0.0)):
         assert attention(p, options=(scale, cap, 0, None)) == 0, (scale, cap)  # (nothing to do: no launch)
+
+
+def test_calls_larger_than_a_launch_are_refused(buffer):
+    """A launch takes fewer than 2^32 threads in a dimension: refused by size before
+    anything is launched, as any other shape."""
+    _, p = buffer
+    lib = fmx.lib()
+    cache = fmx.PagedCache(fmx.FMX_TYPE_BF16, 2, 64, 16, 8, 2048, 128, 64, p, p)
+    for tokens in (1 << 24, 1 << 30, (1 << 31) - 1):
+        batch = fmx.PagedBatch(1, tokens, tokens, 4, p, p, p)
+        turn = fmx.Rope(1, 64, p, 1.0, None)
+        assert lib.fmx_rope_append(ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(turn), 4, 0, p, 512, p, 512, p,
+                                   512, p, 256, p, 256, None) == 3
+    settings = fmx.Sampling(None, None, None, None)
+    for rows in (1 << 23, 1 << 24, (1 << 31) - 1, (1 << 32) - 1):
+        assert lib.fmx_sample(p, 100, rows, 100, ctypes.byref(settings), p, p, None, p, 1 << 62, None) == 3
+    # single tokens of as many sequences: a tile each, and kv heads times that
+    assert attention(p, tokens=1 << 23, sequences=1 << 23) == 3
+    # one prompt: 128 rows a tile, 2 kv heads
+    assert attention(p, tokens=(1 << 29) - 1, max_new=1 << 29) == 3
