@@ -127,7 +127,8 @@ def workspace(bytes_: int = 256, device="cuda") -> torch.Tensor:
 
 def status(ws: torch.Tensor, stream=None) -> int:
     """The error word's status; clears it. Waits for the stream."""
-    return fmx.lib().fmx_moe_status(ws.data_ptr(), fmx.stream_handle(stream))
+    word, handle = _entries(ws, ws.device, 256, torch.uint8), _stream(ws.device, stream)
+    return fmx.lib().fmx_moe_status(word, handle)
 
 
 def rope_append(cache: Cache, batch: Batch, rope: Rope, q, k, v, q_out, ws, positions=None, stream=None):

@@ -104,3 +104,15 @@ def test_calls_larger_than_a_launch_are_refused(buffer):
     assert attention(p, tokens=1 << 23, sequences=1 << 23) == 3
     # one prompt: 128 rows a tile, 2 kv heads
     assert attention(p, tokens=(1 << 29) - 1, max_new=1 << 29) == 3
+
+
+def test_the_status_of_what_is_no_workspace_is_refused(monkeypatch):
+    """The word is cleared by a kernel: it has to be the current GPU's memory."""
+    monkeypatch.setattr(fmx, "lib", lambda: pytest.fail("an address of the host reached the library"))
+    monkeypatch.setattr(fmx, "stream_handle", lambda stream=None: 0)
+    with pytest.raises(ValueError, match="not the current GPU"):
+        sv.status(sv.workspace(device="cpu"))
+    with pytest.raises(ValueError, match="256 entries"):
+        sv.status(torch.zeros(2, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="uint8"):
+        sv.status(torch.zeros(256))
