@@ -835,9 +835,13 @@ uint64_t sample_scratch(uint32_t, uint32_t) { return 0; }
 int sample(const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const fmx_sampling &p,
            const float *uniform, uint32_t *ids, float *probs, uint32_t *status, uint8_t *, hipStream_t s) {
     const SampleArgs A{logits, row_stride, vocab, p, uniform, ids, probs, status};
-    // two workgroups of 512 a CU take turns at what few of their threads do;
-    // where rows leave CUs to themselves, one of 1024
-    const uint32_t threads = rows >= 512 ? kSampleThreads : 1024;
+    // Two workgroups of 512 threads share a CU, one of 1024 fills it: 1024 where
+    // every row has a CU to itself, 512 where rows are more than CUs. us at 1024 / 512
+    // threads, top-p: 64 rows of 131072 54 / 66, 256 of 32001 36.5 / 34.6, 300 58 / 40,
+    // 511 63 / 46, 1000 120 / 86; with top-k, 64 of 131072 24.6 / 27.5, 256 of 32001
+    // 21.6 / 22.4, 300 31 / 22.
+    constexpr uint32_t kCus = 256;
+    const uint32_t threads = rows > kCus ? kSampleThreads : 1024;
     const bool wide = vocab > 4 * threads;
     constexpr uint32_t kMany = kSampleThreads;
     const auto kernel = threads == kMany ? (wide ? sample_kernel<kMany, true> : sample_kernel<kMany, false>)

@@ -168,3 +168,24 @@ def test_extreme_softcaps(gpu, dtype, counts, scale, cap):
         score = (D + 16) * size if abs(scale) <= 1e9 * cap else 8 * cap
         error = (2 * U * score + U * (L + 64)) * spread
         assert ((got[rows] - want).abs() <= error + ref.half_step(F32, want.abs() + error)).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(256, 3000), (257, 3000), (300, 9001), (511, 700), (512, 3000)])
+def test_sampled_rows_do_not_depend_on_how_many_there_are(gpu, rows, vocab):
+    """The number of rows chooses the workgroup: a row's id and probability are the
+    bits they are in a small call."""
+    g = torch.Generator(device=gpu).manual_seed(rows)
+    x = torch.randn(rows, vocab, generator=g, device=gpu) * 2
+    x[::7] = torch.randint(0, 3, x[::7].shape, generator=g, device=gpu).float()
+    u = torch.rand(rows, generator=g, device=gpu)
+    settings = dict(temperature=0.5 + torch.rand(rows, generator=g, device=gpu),
+                    top_k=torch.randint(0, 400, (rows,), generator=g, device=gpu).to(torch.int32),
+                    top_p=0.6 + 0.5 * torch.rand(rows, generator=g, device=gpu),
+                    min_p=0.05 * torch.rand(rows, generator=g, device=gpu))
+    for names in ((), ("top_p",), ("temperature", "top_k"), tuple(settings)):
+        some = {n: settings[n] for n in names}
+        got = sv.sample(x, u, **some)
+        assert sv.status(got.ws) == 0
+        for at in range(0, rows, 50):
+            few = sv.sample(x[at:at + 50], u[at:at + 50], **{n: t[at:at + 50] for n, t in some.items()})
+            assert torch.equal(few.ids, got.ids[at:at + 50]) and torch.equal(few.probs, got.probs[at:at + 50]), (names, at)
