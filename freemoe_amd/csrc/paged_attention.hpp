@@ -822,19 +822,21 @@ template <uint32_t N> __device__ __forceinline__ void wait_and_barrier() {
 // number for each block (behind the last one it loads that again), so that a
 // count of outstanding operations tells which blocks have landed.
 // kGrouped: the rows of a load instruction lie in one page (blocks start at
-// multiples of 8, and the page size is one of their number), less than 2^30
-// bytes apart.
+// multiples of 8 or of the page size, which is one of their number), less than
+// 2^30 bytes apart. (A prompt of 4096, bf16: 159 us; pages of 6, 5 and 1 positions,
+// whose rows are looked up one by one, 178, 180 and 195.)
 // Bound by the matrix cores and the SIMDs' issue between their products: 32 rows
 // a wavefront halve the LDS reads per product against 16, two workgroups share a
 // CU, and while one wavefront of a SIMD forms its weights the other's products
-// run. 2048 tokens at the end of 16384 positions, 32 / 8 heads of 128, bf16: 530
-// us, 0.97 PFLOP/s counted as two products per visible pair (a library product
-// of 8192^3 reaches 1.14); a prompt of 4096: 160 us, 0.86; head_dim 256 keeps one
-// workgroup a CU for its registers, 0.53; f32, a ragged batch of 2544 tokens with
-// a window of 1000, 16 / 8 heads of 96: 190 us, 65 TFLOP/s of the 153 a library
-// product reaches: the tiles' unequal lengths leave CUs idle for a third of it.
-// Of the 530 us, left out in a copy: the exponentials 35, the keys' LDS reads
-// 35, the loads 70, three quarters of the value products 120.
+// run. 2048 tokens at the end of 16384 positions, 32 / 8 heads of 128, bf16: 531 to
+// 559 us on different cards, 0.97 to 0.92 PFLOP/s counted as two products per
+// visible pair (a library product of 8192^3 reaches 1.14); a prompt of 4096: 159 to
+// 166 us, 0.86 to 0.83; head_dim 256 (16 / 8 heads) keeps one workgroup a CU for its
+// registers, 266 us, 0.52; f32, a ragged batch of 2544 tokens with a window of 1000,
+// 16 / 8 heads of 96: 190 us, 65 TFLOP/s of the 153 a library product reaches: the
+// tiles' unequal lengths leave CUs idle for a third of it. Of the chunk's time (531
+// us), left out in a copy: the exponentials 35, the keys' LDS reads 35, the loads
+// 70, three quarters of the value products 120.
 // grid: row tiles x splits x kv heads, the heads fastest; the tiles with the
 // most keys first.
 template <typename T, int DP, int DC, int kParts, bool kGrouped>
@@ -1132,9 +1134,11 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs 
 // Workgroups that a split aims at; an f32 call, whose blocks take 16 times as
 // long, aims at kFillLong where the pieces stay of kLongPiece keys and more, so
 // that tiles of unequal length end together. (us at 512 / 1280: f32, 11 new tokens
-// of 4 sequences over up to 60376 positions, 2 kv heads, 363 / 264; 709 over 1512,
-// 8 heads, whose pieces are shorter, 71 / 77; bf16, a prompt of 4096 tokens, 8
-// heads, 182 / 227, for the sums' way through memory.)
+// of 4 sequences over up to 60376 positions, 2 kv heads, 352 / 259; a ragged batch
+// of 2544 with a window of 1000, 8 kv heads, 198 / 190; 709 over 1512, 8 heads,
+// whose pieces would be shorter than kLongPiece and which so stays at 512, 67 / 75;
+// bf16, a prompt of 4096 tokens, 8 kv heads, 159 / 209, for the sums' way through
+// memory.)
 constexpr uint32_t kFillRows = 2048, kFillTiles = 512, kFillLong = 1280, kLongPiece = 256;
 // Rows of a sequence up to which the 16-row kernel takes a call. 32, 64 and 128
 // rows of 16 sequences over 4096 positions, 8 kv heads of 128, 16-row / 128-row

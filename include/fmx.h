@@ -340,10 +340,12 @@ typedef struct fmx_paged_batch {
     const uint32_t *table;
 } fmx_paged_batch;
 
-/* The error word of the calls below is the first of their workspace, as for
- * the MoE calls, but they only add to it: zeroed with the workspace (fmx_alloc
- * does) and by fmx_moe_status, it holds what any call since then met, so a
- * program reads it once per step. A workspace serves one call at a time. */
+/* The error word of the calls below is the first of their workspace. They only
+ * add to it: zeroed with the workspace (fmx_alloc does) and by fmx_moe_status, it
+ * holds what any of them met since then, so a program reads it once per step. The
+ * MoE calls and fmx_attention_decode clear the word of theirs when they start: a
+ * workspace that one of these takes as well loses what was reported before, so
+ * they are given another one. A workspace serves one call at a time. */
 
 /* Rotary positions. */
 enum { FMX_ROPE_INTERLEAVED = 0,  /* pairs (2c, 2c + 1) */
@@ -445,7 +447,11 @@ typedef struct fmx_sampling {
  * the same in whatever order they are added, so a row's token depends on
  * nothing but its inputs; w comes from double arithmetic from about 1/8 of the
  * largest on and next to min_p's border, else from a float's exponential
- * (a weight of 2^t to within (2 |t| + 2) 2^-24 of itself). Logits of -inf are never chosen. A row with a NaN or
+ * (a weight of 2^t to within (2 |t| + 2) 2^-24 of itself): where the border of a
+ * filter or of a token's share lies nearer to its target than these errors add up
+ * to, the neighbour beyond it may be taken. Logits of
+ * -inf, and those further below the largest than a float reaches (3.4e38), are
+ * never chosen. A row with a NaN or
  * +inf or without a finite logit, a temperature below 0, a NaN setting or uniform gives
  * ids[row] = 0xffffffff, probs[row] = 0 and FMX_ERR_INTERNAL from
  * fmx_moe_status. vocab <= 262144, rows below 2^23. */
