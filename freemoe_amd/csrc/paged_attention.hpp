@@ -399,8 +399,8 @@ template <int DP> struct Tile16<float, DP> {
 // tanhf's instructions. Which of the two a score takes goes by that score alone,
 // whatever the others of the wavefront are (keys its row does not see among
 // them); their vote only decides whether tanhf has to be computed at all. (A
-// prompt of 4096 in bf16: 170 us without a cap, 223 with scores of a thirtieth of
-// it, 430 with scores about as large as it.)
+// prompt of 4096 in bf16: 159 us without a cap, 196 with scores of a thirtieth of
+// it, 420 with scores about as large as it.)
 template <class Scores> __device__ __forceinline__ void cap_scores(const AttentionArgs &A, Scores &s) {
     constexpr int kN = sizeof(Scores) / sizeof(float);
     if (A.softcap == 0.0f) return;
