@@ -282,9 +282,8 @@ def _plain_rope(s):
         pair = torch.stack((a * cos - b * sin, a * sin + b * cos), dim=-1).flatten(-2)
         turned = torch.cat((pair, rot[..., R:]), dim=-1)
     s["q_out"].copy_(torch.where(owned[:, None, None], turned[:, :H].to(s["q_out"].dtype), s["q_out"]))
-    n = T - SPARE
-    page = s["table"].long()[seq, position // ps]
-    at = (page[:n], position[:n] % ps)
+    n = T - SPARE  # (the rows behind the last sequence have no place in the table)
+    at = (s["table"].long()[seq[:n], position[:n] // ps], position[:n] % ps)
     _by_position(c, s["k"])[at] = turned[:n, H:].to(s["k"].dtype)
     _by_position(c, s["v"])[at] = x[:n, H + kvh:].to(s["v"].dtype)
     return {"q": s["q_out"], "k": s["k"], "v": s["v"]}
